@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/homura_rocm.h.
+"""ctypes binding of the C ABI in include/homura_rocm.h and include/homura_nn.h.
 
 This is the thinnest possible caller of libhomura_rocm.so: the structs, the prototypes and a few
 conveniences (contexts, device buffers, status -> exception). It is what the parity tests and
@@ -122,6 +122,22 @@ PROTOTYPES = {
     "hmr_ext_stream": (c_int32, [CTX, POINTER(c_void_p)]),
 }
 
+# libhomura_nn: exactly the declarations of include/homura_nn.h.
+NN_PROTOTYPES = {
+    "hmn_last_error": (c_char_p, []),
+    "hmn_recurrence_workspace": (c_int32, [DESC_P, POINTER(c_int64)]),
+    "hmn_recurrence": (c_int32, [CTX, c_int32] + [DESC_P] * 6 + [c_void_p, c_int64]),
+    "hmn_recurrence_backward": (c_int32, [CTX, c_int32] + [DESC_P] * 10 + [c_void_p, c_int64]),
+    "hmn_group_norm_workspace": (c_int32, [DESC_P, c_int64, c_int32, POINTER(c_int64)]),
+    "hmn_group_norm": (c_int32, [CTX] + [DESC_P] * 6 + [c_int64, c_double, c_int32, c_void_p, c_int64]),
+    "hmn_group_norm_backward": (c_int32, [CTX] + [DESC_P] * 9 + [c_int64, c_int32, c_void_p, c_int64]),
+    "hmn_dropout": (c_int32, [CTX, DESC_P, DESC_P, DESC_P, c_double, c_uint64, c_uint64, c_void_p]),
+}
+
+# The recurrence's forms and the activations of hmn_group_norm.
+GATE_FACTOR, GATE_SIGMOID = 0, 1
+ACTIVATION = {"none": -1, **{name: UNARY[name] for name in ("relu", "silu", "gelu", "gelu_tanh")}}
+
 # Exported stubs of other kernel families (include/homura_rocm_unbuilt.h); bound without prototypes.
 UNBUILT = [
     "hmr_max_pool2d_backward_workspace", "hmr_max_pool2d_backward", "hmr_max_pool2d",
@@ -132,6 +148,7 @@ UNBUILT = [
 ]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libhomura_rocm.so")
+NN_PATH = os.path.join(os.path.dirname(LIB_PATH), "libhomura_nn.so")
 
 
 class HmrError(RuntimeError):
@@ -141,14 +158,14 @@ class HmrError(RuntimeError):
         self.message = message
 
 
-def load(path: str = LIB_PATH) -> ctypes.CDLL:
-    """Loads libhomura_rocm.so and declares every prototype. Raises if the library is absent."""
+def load(path: str = LIB_PATH, prototypes=PROTOTYPES) -> ctypes.CDLL:
+    """Loads libhomura_rocm.so (or the library at `path`) and declares every prototype. Raises if it is absent."""
     if not os.path.exists(path):
         raise ImportError(
             f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
             "(or `make -C homura_amd/csrc`). There is no fallback implementation.")
     lib = ctypes.CDLL(path)
-    for name, (restype, argtypes) in PROTOTYPES.items():
+    for name, (restype, argtypes) in prototypes.items():
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes
@@ -156,11 +173,18 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 
 lib = load()
+nn = load(NN_PATH, NN_PROTOTYPES)
 
 
 def check(status: int) -> None:
     if status != HMR_OK:
         raise HmrError(status, lib.hmr_last_error().decode("utf-8", "replace"))
+
+
+def check_nn(status: int) -> None:
+    """check() for the calls of libhomura_nn, which keeps its own failure text."""
+    if status != HMR_OK:
+        raise HmrError(status, nn.hmn_last_error().decode("utf-8", "replace"))
 
 
 def make_desc(ptr: int, dtype: int, sizes=(), strides=(), offset: int = 0) -> hmr_tensor_desc:

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "homura.hpp"
+#include "homura_nn.h"
 #include "homura_rocm.h"
 #include "homura_rocm_ext.h"
 
@@ -1057,6 +1058,109 @@ std::optional<uint64_t> random_int_batch(const TensorData &out, uint64_t seed, u
     std::lock_guard<std::recursive_mutex> lock(st.exec);
     expect(hmr_copy_to_host(st.ctx, &count, static_cast<const char *>(ws) + 2 * tiles * sizeof(int64_t), sizeof count));
     return static_cast<uint64_t>(count);
+}
+
+// ---- libhomura_nn -----------------------------------------------------------------------------------------
+
+namespace {
+
+void expect_nn(hmr_status s) {
+    if (s == HMR_OK) return;
+    std::string message = hmn_last_error();
+    if (s == HMR_OUT_OF_MEMORY) throw Error("ROCm out of memory: " + message);
+    throw Error(message);
+}
+
+// The operand as it is, without merging dimensions: the entry points tell them apart.
+hmr_tensor_desc whole_desc(const TensorData &t) {
+    hmr_tensor_desc d;
+    std::memset(&d, 0, sizeof d);
+    d.data = t.storage->ptr();
+    d.offset = t.layout.offset;
+    d.dtype = static_cast<int32_t>(t.dtype);
+    d.ndim = static_cast<int32_t>(t.layout.shape.size());
+    for (size_t k = 0; k < t.layout.shape.size(); ++k) {
+        d.sizes[k] = t.layout.shape[k];
+        d.strides[k] = t.layout.strides[k];
+    }
+    return d;
+}
+
+// A description that may be absent.
+struct MaybeDesc {
+    explicit MaybeDesc(const TensorData *t) : there(t != nullptr) {
+        if (t) d = whole_desc(*t);
+    }
+    const hmr_tensor_desc *get() const { return there ? &d : nullptr; }
+    bool there;
+    hmr_tensor_desc d;
+};
+
+int32_t activation_code(std::optional<UnaryOp> activation) {
+    return activation ? static_cast<int32_t>(*activation) : HMN_ACTIVATION_NONE;
+}
+
+}  // namespace
+
+void recurrence(bool sigmoid, const TensorData &out, const TensorData &last, const TensorData &gate, const TensorData &input,
+                const TensorData *initial, const TensorData *lengths) {
+    const hmr_tensor_desc o = whole_desc(out), l = whole_desc(last), g = whole_desc(gate), x = whole_desc(input);
+    const MaybeDesc i(initial), n(lengths);
+    int64_t bytes = 0;
+    expect_nn(hmn_recurrence_workspace(&g, &bytes));
+    auto ws = workspace(bytes, gate.device());
+    exec(out, [&](hmr_context_t ctx) {
+        expect_nn(hmn_recurrence(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &o, &l, &g, &x, i.get(), n.get(),
+                                 ws ? ws->ptr() : nullptr, bytes));
+    });
+}
+
+void recurrence_backward(bool sigmoid, const TensorData &d_gate, const TensorData &d_input, const TensorData &d_initial,
+                         const TensorData &g, const TensorData *g_last, const TensorData &gate, const TensorData &input,
+                         const TensorData &out, const TensorData *initial, const TensorData *lengths) {
+    const hmr_tensor_desc dg = whole_desc(d_gate), dx = whole_desc(d_input), di = whole_desc(d_initial), gr = whole_desc(g);
+    const hmr_tensor_desc z = whole_desc(gate), x = whole_desc(input), h = whole_desc(out);
+    const MaybeDesc gl(g_last), i(initial), n(lengths);
+    int64_t bytes = 0;
+    expect_nn(hmn_recurrence_workspace(&z, &bytes));
+    auto ws = workspace(bytes, gate.device());
+    exec(out, [&](hmr_context_t ctx) {
+        expect_nn(hmn_recurrence_backward(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &dg, &dx, &di, &gr, gl.get(), &z, &x, &h,
+                                          i.get(), n.get(), ws ? ws->ptr() : nullptr, bytes));
+    });
+}
+
+void group_norm(const TensorData &out, const TensorData &mean, const TensorData &rstd, const TensorData &src, const TensorData *weight,
+                const TensorData *bias, int64_t groups, double eps, std::optional<UnaryOp> activation) {
+    const hmr_tensor_desc o = whole_desc(out), m = whole_desc(mean), r = whole_desc(rstd), s = whole_desc(src);
+    const MaybeDesc w(weight), b(bias);
+    int64_t bytes = 0;
+    expect_nn(hmn_group_norm_workspace(&s, groups, 0, &bytes));
+    auto ws = workspace(bytes, src.device());
+    exec(out, [&](hmr_context_t ctx) {
+        expect_nn(hmn_group_norm(ctx, &o, &m, &r, &s, w.get(), b.get(), groups, eps, activation_code(activation),
+                                 ws ? ws->ptr() : nullptr, bytes));
+    });
+}
+
+void group_norm_backward(const TensorData &d_src, const TensorData *d_weight, const TensorData *d_bias, const TensorData &g,
+                         const TensorData &src, const TensorData &mean, const TensorData &rstd, const TensorData *weight,
+                         const TensorData *bias, int64_t groups, std::optional<UnaryOp> activation) {
+    const hmr_tensor_desc ds = whole_desc(d_src), gr = whole_desc(g), s = whole_desc(src), m = whole_desc(mean), r = whole_desc(rstd);
+    const MaybeDesc dw(d_weight), db(d_bias), w(weight), b(bias);
+    int64_t bytes = 0;
+    expect_nn(hmn_group_norm_workspace(&s, groups, 1, &bytes));
+    auto ws = workspace(bytes, src.device());
+    exec(d_src, [&](hmr_context_t ctx) {
+        expect_nn(hmn_group_norm_backward(ctx, &ds, dw.get(), db.get(), &gr, &s, &m, &r, w.get(), b.get(), groups,
+                                          activation_code(activation), ws ? ws->ptr() : nullptr, bytes));
+    });
+}
+
+void dropout(const TensorData &out, const TensorData &src, const TensorData *residual, const DropoutMask &mask) {
+    const hmr_tensor_desc o = whole_desc(out), s = whole_desc(src);
+    const MaybeDesc r(residual);
+    exec(out, [&](hmr_context_t ctx) { expect_nn(hmn_dropout(ctx, &o, &s, r.get(), mask.p, mask.seed, mask.offset, nullptr)); });
 }
 
 void upload(const TensorData &dst, const TensorData &src) {

@@ -379,10 +379,63 @@ Tensor var_std(const Tensor &g, const Tensor &x, const std::optional<Tensor> &st
 Tensor softmax(const Tensor &g, const Tensor &y, int64_t dim, bool log);
 }  // namespace grad
 
+// Operators of sequence models' recurrent blocks (the reference has no counterpart; homura_nn.h states what each one
+// computes). They run on ROCm tensors only.
+struct RecurrenceStates {
+    Tensor out;   // every state, as `input`
+    Tensor last;  // the state after the last step
+};
+// h_t = gate_t h_{t-1} + input_t (or, `sigmoid`, a_t h_{t-1} + (1 - a_t) input_t with a = sigmoid(gate)) along
+// dimension 1 of input [B, T, ...]; the gate is broadcast to the input's shape. `initial` is [B, ...], zero without one;
+// `lengths` (I32 or I64, [B]) the sequences' own numbers of steps. `last` is F32 for F16 and BF16 sequences, unless
+// `initial` is of their type.
+RecurrenceStates linear_recurrence(const Tensor &gate, const Tensor &input, const std::optional<Tensor> &initial,
+                                   const std::optional<Tensor> &lengths, bool sigmoid);
+struct NormOutput {
+    Tensor out;
+    Tensor mean, rstd;  // [N, groups], F32 (F64 for F64)
+};
+// Group normalisation of x [N, ..., C] over equal runs of its last dimension, then the activation (Relu, Silu, Gelu or
+// GeluTanh) if there is one.
+NormOutput group_norm(const Tensor &x, int64_t groups, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias,
+                      double eps, std::optional<UnaryOp> activation);
+// What a dropout's mask is a function of, besides the position: kept for the backward pass instead of the mask.
+struct DropoutMask {
+    double p = 0.0;
+    uint64_t seed = 0, offset = 0;
+};
+struct DropoutOutput {
+    Tensor out;
+    DropoutMask mask;
+};
+// residual + (kept ? x / (1 - p) : 0), the mask drawn from the process-wide generator.
+DropoutOutput dropout(const Tensor &x, double p, const std::optional<Tensor> &residual);
+Tensor dropout_with(const Tensor &x, const DropoutMask &mask, const std::optional<Tensor> &residual);
+namespace grad {
+struct Recurrence {
+    Tensor d_gate, d_input;  // d_gate has the gate's own shape: summed over what it was broadcast over
+    Tensor d_initial;
+};
+// For the gradients of out and last (either may be absent).
+Recurrence linear_recurrence(const std::optional<Tensor> &g, const std::optional<Tensor> &g_last, const Tensor &gate,
+                             const Tensor &input, const Tensor &out, const std::optional<Tensor> &initial,
+                             const std::optional<Tensor> &lengths, bool sigmoid);
+struct Norm {
+    Tensor d_x;
+    std::optional<Tensor> d_weight, d_bias;  // where there is a weight, a bias
+};
+Norm group_norm(const Tensor &g, const Tensor &x, const Tensor &mean, const Tensor &rstd, int64_t groups,
+                const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, std::optional<UnaryOp> activation);
+// The gradient of x; the residual's is g itself.
+Tensor dropout(const Tensor &g, const DropoutMask &mask);
+}  // namespace grad
+
 // Random sampling from the process-wide Philox4x32-10 generator, shared by all devices: a GPU computes the
 // CPU's uniform samples and integers bit for bit, also when calls on the two alternate
 // (ref: src/ops/random.rs). `uniform` and `normal` are what `uniform_` / `normal_` fill a tensor with.
 void manual_seed(uint64_t seed);
+// Takes `blocks` Philox blocks from the generator: its seed and the first block's number.
+void reserve_random_blocks(uint64_t blocks, uint64_t &seed, uint64_t &start);
 Tensor rand(const Shape &shape, DType dtype, Device device);
 Tensor randn(const Shape &shape, DType dtype, Device device);
 Tensor randint(int64_t low, int64_t high, const Shape &shape, DType dtype, Device device);
@@ -496,6 +549,19 @@ void random_uniform(const TensorData &out, uint64_t seed, uint64_t offset, doubl
 void random_normal(const TensorData &out, uint64_t seed, uint64_t offset, double mean, double std);
 std::optional<uint64_t> random_int_batch(const TensorData &out, uint64_t seed, uint64_t offset, uint64_t blocks, int64_t low,
                                          uint64_t range, uint64_t threshold, const TensorData *workspace);
+// The entry points of libhomura_nn. Sequences are [B, T, C], states [B, C], maps [N, S, C]; a null pointer is an operand
+// that is not there.
+void recurrence(bool sigmoid, const TensorData &out, const TensorData &last, const TensorData &gate, const TensorData &input,
+                const TensorData *initial, const TensorData *lengths);
+void recurrence_backward(bool sigmoid, const TensorData &d_gate, const TensorData &d_input, const TensorData &d_initial,
+                         const TensorData &g, const TensorData *g_last, const TensorData &gate, const TensorData &input,
+                         const TensorData &out, const TensorData *initial, const TensorData *lengths);
+void group_norm(const TensorData &out, const TensorData &mean, const TensorData &rstd, const TensorData &src, const TensorData *weight,
+                const TensorData *bias, int64_t groups, double eps, std::optional<UnaryOp> activation);
+void group_norm_backward(const TensorData &d_src, const TensorData *d_weight, const TensorData *d_bias, const TensorData &g,
+                         const TensorData &src, const TensorData &mean, const TensorData &rstd, const TensorData *weight,
+                         const TensorData *bias, int64_t groups, std::optional<UnaryOp> activation);
+void dropout(const TensorData &out, const TensorData &src, const TensorData *residual, const DropoutMask &mask);
 // Host <-> device and device <-> host transfers of contiguous data of one dtype.
 void upload(const TensorData &dst, const TensorData &src);
 void download(const TensorData &dst, const TensorData &src);

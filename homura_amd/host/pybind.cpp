@@ -122,6 +122,60 @@ PYBIND11_MODULE(_host, m) {
     m.def("grad_extremum_dim", &grad::extremum_dim);
     m.def("grad_var_std", &grad::var_std);
     m.def("grad_softmax", &grad::softmax);
+    // The operators of recurrent blocks. An activation is the name of its unary op, or None.
+    auto activation = [](const std::optional<std::string> &name) -> std::optional<UnaryOp> {
+        if (!name) return std::nullopt;
+        for (const auto &[n, op] : {std::pair<const char *, UnaryOp>{"relu", UnaryOp::Relu}, {"silu", UnaryOp::Silu}, {"gelu", UnaryOp::Gelu},
+                                    {"gelu_tanh", UnaryOp::GeluTanh}}) {
+            if (*name == n) return op;
+        }
+        throw Error("unknown activation '" + *name + "'");
+    };
+    m.def("linear_recurrence",
+          [](const Tensor &gate, const Tensor &input, const std::optional<Tensor> &initial, const std::optional<Tensor> &lengths, bool sigmoid) {
+              RecurrenceStates r = linear_recurrence(gate, input, initial, lengths, sigmoid);
+              return py::make_tuple(r.out, r.last);
+          },
+          py::arg("gate"), py::arg("input"), py::arg("initial") = py::none(), py::arg("lengths") = py::none(), py::arg("sigmoid") = false);
+    m.def("grad_linear_recurrence",
+          [](const std::optional<Tensor> &g, const std::optional<Tensor> &g_last, const Tensor &gate, const Tensor &input, const Tensor &out,
+             const std::optional<Tensor> &initial, const std::optional<Tensor> &lengths, bool sigmoid) {
+              grad::Recurrence r = grad::linear_recurrence(g, g_last, gate, input, out, initial, lengths, sigmoid);
+              return py::make_tuple(r.d_gate, r.d_input, r.d_initial);
+          },
+          py::arg("g"), py::arg("g_last"), py::arg("gate"), py::arg("input"), py::arg("out"), py::arg("initial") = py::none(),
+          py::arg("lengths") = py::none(), py::arg("sigmoid") = false);
+    m.def("group_norm",
+          [activation](const Tensor &x, int64_t groups, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, double eps,
+                       const std::optional<std::string> &act) {
+              NormOutput r = group_norm(x, groups, weight, bias, eps, activation(act));
+              return py::make_tuple(r.out, r.mean, r.rstd);
+          },
+          py::arg("x"), py::arg("groups"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5,
+          py::arg("activation") = py::none());
+    m.def("grad_group_norm",
+          [activation](const Tensor &g, const Tensor &x, const Tensor &mean, const Tensor &rstd, int64_t groups,
+                       const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, const std::optional<std::string> &act) {
+              grad::Norm r = grad::group_norm(g, x, mean, rstd, groups, weight, bias, activation(act));
+              return py::make_tuple(r.d_x, r.d_weight, r.d_bias);
+          },
+          py::arg("g"), py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("groups"), py::arg("weight") = py::none(),
+          py::arg("bias") = py::none(), py::arg("activation") = py::none());
+    // A dropout's mask travels as (p, seed, offset).
+    m.def("dropout",
+          [](const Tensor &x, double p, const std::optional<Tensor> &residual) {
+              DropoutOutput r = dropout(x, p, residual);
+              return py::make_tuple(r.out, py::make_tuple(r.mask.p, r.mask.seed, r.mask.offset));
+          },
+          py::arg("x"), py::arg("p"), py::arg("residual") = py::none());
+    m.def("dropout_with",
+          [](const Tensor &x, const std::tuple<double, uint64_t, uint64_t> &mask, const std::optional<Tensor> &residual) {
+              return dropout_with(x, DropoutMask{std::get<0>(mask), std::get<1>(mask), std::get<2>(mask)}, residual);
+          },
+          py::arg("x"), py::arg("mask"), py::arg("residual") = py::none());
+    m.def("grad_dropout", [](const Tensor &g, const std::tuple<double, uint64_t, uint64_t> &mask) {
+        return grad::dropout(g, DropoutMask{std::get<0>(mask), std::get<1>(mask), std::get<2>(mask)});
+    });
     m.def("manual_seed", &manual_seed);
     m.def("rand", [](const Shape &shape, DType d, const std::string &dev) { return rand(shape, d, parse_device(dev)); },
           py::arg("shape"), py::arg("dtype") = DType::F32, py::arg("device") = "cpu");

@@ -146,6 +146,8 @@ Tensor random_tensor(const Shape &shape, DType dtype, Device device, const Dist 
 
 }  // namespace
 
+void reserve_random_blocks(uint64_t blocks, uint64_t &seed, uint64_t &start) { reserve_blocks(blocks, seed, start); }
+
 void manual_seed(uint64_t seed) {
     std::lock_guard<std::mutex> lock(g_lock);
     g_generator.seed = seed;
