@@ -64,6 +64,96 @@ inline hmr_status check_room(const char *who, const void *workspace, int64_t hav
 
 // ---- device side --------------------------------------------------------------------------------------------------
 
+// V elements of type T as memory holds them, moved in accesses of up to 16 bytes. The vectors need no more alignment than
+// an element has (global accesses of this target take any), so a row of odd length or an odd start costs a few split
+// lines, not another kernel.
+template <class T, int V>
+struct Vec {
+    using C = typename Comp<T>::C;
+    static constexpr int kBytes = V * static_cast<int>(sizeof(T)), kWords = kBytes < 4 ? 1 : kBytes / 4;
+    static constexpr int kWide = kWords % 4 == 0 ? 4 : (kWords % 2 == 0 ? 2 : 1);  // words of an access
+    typedef uint32_t Access __attribute__((ext_vector_type(kWide), aligned(sizeof(T) < 4 ? sizeof(T) : 4)));
+    static_assert(kBytes == 2 || kBytes % 4 == 0, "whole words, or one half");
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (kBytes == 2) {
+            w[0] = *reinterpret_cast<const uint16_t *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords / kWide; ++i) {
+                const Access x = reinterpret_cast<const Access *>(p)[i];
+#pragma unroll
+                for (int k = 0; k < kWide; ++k) w[i * kWide + k] = x[k];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (kBytes == 2) {
+            *reinterpret_cast<uint16_t *>(p) = static_cast<uint16_t>(w[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords / kWide; ++i) {
+                Access x;
+#pragma unroll
+                for (int k = 0; k < kWide; ++k) x[k] = w[i * kWide + k];
+                reinterpret_cast<Access *>(p)[i] = x;
+            }
+        }
+    }
+    // Element i in the computation type.
+    __device__ __forceinline__ C get(int i) const {
+        if constexpr (std::is_same_v<T, float>) {
+            return bits_as<float>(w[i]);
+        } else if constexpr (std::is_same_v<T, double>) {
+            return bits_as<double>((static_cast<uint64_t>(w[2 * i + 1]) << 32) | w[2 * i]);
+        } else if constexpr (std::is_same_v<T, bf16_t>) {
+            return bits_as<float>(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xFFFF0000u);
+        } else {
+            return Comp<T>::up(T{static_cast<uint16_t>(i % 2 == 0 ? w[i / 2] : w[i / 2] >> 16)});
+        }
+    }
+    // Computation-type values rounded into the vector.
+    __device__ __forceinline__ void round(const C (&x)[V]) {
+        if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = bits_as<uint32_t>(x[i]);
+        } else if constexpr (std::is_same_v<T, double>) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const uint64_t b = bits_as<uint64_t>(x[i]);
+                w[2 * i] = static_cast<uint32_t>(b), w[2 * i + 1] = static_cast<uint32_t>(b >> 32);
+            }
+        } else if constexpr (V == 1) {
+            w[0] = Comp<T>::down(x[0]).bits;
+        } else if constexpr (std::is_same_v<T, bf16_t>) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) w[i / 2] = bf16_round_pair(x[i], x[i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) w[i / 2] = f16_round(x[i]).bits | (static_cast<uint32_t>(f16_round(x[i + 1]).bits) << 16);
+        }
+    }
+    // Every element x (a value the type holds).
+    __device__ __forceinline__ void fill(C x) {
+        C all[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) all[i] = x;
+        round(all);
+    }
+    // The vector as it is, or all zeros.
+    __device__ __forceinline__ void only(bool as_it_is) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = as_it_is ? w[i] : 0;
+    }
+    // Makes the compiler forget what it knows of the words, so that what was computed from them is computed again where
+    // it is used again instead of being kept in registers meanwhile.
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+    }
+};
+
 // One element of a tensor whose type is the computation type or, at run time, a narrower one.
 template <class T>
 __device__ __forceinline__ typename Comp<T>::C load_state(const char *p, int64_t at, bool wide) {

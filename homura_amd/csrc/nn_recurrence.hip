@@ -6,6 +6,12 @@ namespace nn {
 namespace {
 
 // ---- one thread per channel ----------------------------------------------------------------------------------
+//
+// Decoding and other sequences of a few steps: nothing to fold, one launch, the states in registers. Also steps so far apart
+// that a tile of the scan spans more than its 32-bit offsets (2 million elements of 16 bits: time-major batches with as
+// many channels in all, which keep the memory busy a thread each). `last` may be
+// `initial`: a channel's state is read and written by its own thread.
+constexpr int64_t kFewSteps = 4;
 
 template <class T, int FORM>
 __global__ void __launch_bounds__(kBlock) forward_kernel(RecurrenceArgs a) {
@@ -100,6 +106,23 @@ RecurrenceArgs batch_args(const hmr_tensor_desc *gate, const hmr_tensor_desc *le
     return a;
 }
 
+// Whether every operand's channels lie next to each other.
+bool adjacent(std::initializer_list<const hmr_tensor_desc *> operands) {
+    for (const hmr_tensor_desc *d : operands) {
+        if (d->strides[2] != 1) return false;
+    }
+    return true;
+}
+
+// Whether a tile of the scan's largest shape spans less than 2^31 bytes in every operand.
+bool near_by(std::initializer_list<const hmr_tensor_desc *> operands) {
+    for (const hmr_tensor_desc *d : operands) {
+        const int64_t most = (int64_t{1} << 30) / dtype_size(d->dtype);
+        if (d->strides[1] > most / (kMostSteps + 1) || d->strides[2] > most / kMostChannels) return false;
+    }
+    return true;
+}
+
 uint32_t grid_of(hmr_context_t ctx, const RecurrenceArgs &a) {
     const int64_t groups = (a.B * a.C + kBlock - 1) / kBlock, most = int64_t{64} * ctx->compute_units;
     return static_cast<uint32_t>(groups < most ? groups : most);
@@ -121,6 +144,10 @@ hmr_status forward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *out, 
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
+            if (a.T > kFewSteps && near_by({gate, input, out})) {
+                queue_scan_forward(stream, gate->dtype, form, a, adjacent({gate, input, out}), workspace);
+                return;
+            }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {
                 forward_kernel<T, decltype(f)::value><<<grid_of(ctx, a), kBlock, 0, stream>>>(a);
             });
@@ -152,6 +179,10 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
+            if (a.T > kFewSteps && near_by({gate, input, out, grad, d_gate, d_input})) {
+                queue_scan_backward(stream, gate->dtype, form, a, adjacent({gate, input, out, grad, d_gate, d_input}), workspace);
+                return;
+            }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {
                 backward_kernel<T, decltype(f)::value><<<grid_of(ctx, a), kBlock, 0, stream>>>(a);
             });
@@ -160,9 +191,6 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
 }
 
 }  // namespace
-
-// The one thread per channel keeps its state in a register.
-int64_t room_for(const hmr_tensor_desc *) { return 0; }
 
 }  // namespace nn
 }  // namespace hmr

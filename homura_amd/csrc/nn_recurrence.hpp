@@ -95,7 +95,70 @@ __device__ __forceinline__ C step_back(C gate, C input, C g, C before, C &d_gate
     }
 }
 
-// Bytes of workspace of either direction.
+// ---- the scan ------------------------------------------------------------------------------------------------------
+//
+// Along the direction of processing (q = t forwards, T - 1 - t backwards) every step maps the running value e to
+// f e + u: forwards e is the state, f the factor and u the addend; backwards e is the gradient that is handed back,
+// f = a_t and u = a_t grad_t. A stretch of steps maps e to F e + U, so stretches fold in any grouping, and each is read
+// once: a workgroup holds a tile of R * S steps x L * V channels in registers (lane (r, l) has the S steps from r * S on of
+// V channels), folds its steps, then the R slots through LDS, gets the value that enters the tile, and runs its steps
+// again from there with the inputs still in registers.
+//
+// Where the value that enters a tile comes from:
+//   walk   a workgroup goes through all the tiles of its channels in order, the next tile's loads under way while this
+//          one is worked on. Nothing is shared between workgroups. For batches with many channels in all.
+//   chain  a workgroup per tile. Tiles publish their (F, U) in the workspace and each folds what it needs in a fixed
+//          order: the tiles before it in its group of about sqrt(tiles), and the groups before that. So that every wait
+//          ends, tiles are numbered by a ticket that a workgroup draws as it starts, and wait for smaller tickets only:
+//          their workgroups run already, and publish before they wait. An entry is one 64-bit word (two in f64), written
+//          and polled with relaxed device-scope atomics, so that no cache has to be flushed; the launch before fills the
+//          workspace with words that no entry is.
+struct ScanPlan {
+    int64_t blocks;  // of channels
+    int64_t tiles;   // along the sequence
+    int64_t chains;  // B * blocks
+    int64_t group;   // tiles of a group
+    bool walk;
+};
+
+constexpr int kScanBlock = 256;
+
+template <class T, int V, int R, int S>
+struct ScanShape {
+    static constexpr int kLanes = kScanBlock / R, kChannels = kLanes * V, kSteps = R * S;
+    // Chains from which on a workgroup per chain keeps the memory busy.
+    static constexpr int64_t kWalkChains = 512;
+    static constexpr int kWords = sizeof(typename Comp<T>::C) / 4;  // 64-bit words of an entry
+
+    static ScanPlan plan(int64_t B, int64_t steps, int64_t C) {
+        ScanPlan p{};
+        p.blocks = (C + kChannels - 1) / kChannels;
+        p.tiles = (steps + kSteps - 1) / kSteps;
+        p.chains = B * p.blocks;
+        p.walk = p.tiles <= 1 || p.chains >= kWalkChains;
+        p.group = 1;
+        while (p.group * p.group < p.tiles) ++p.group;
+        return p;
+    }
+    static int64_t entries(const ScanPlan &p) { return p.chains * (p.tiles + p.tiles / p.group + 1) * kChannels; }
+    // 64-bit words of workspace: the ticket's, then the tiles' entries, then the groups'.
+    static int64_t words(const ScanPlan &p) { return p.walk ? 0 : 8 + entries(p) * kWords; }
+};
+
+struct ScanArgs {
+    RecurrenceArgs a;
+    ScanPlan p;
+    uint64_t *room;
+};
+
+// The largest tile of any shape in use.
+constexpr int64_t kMostSteps = 256, kMostChannels = 256;
+
+// Queue the scan of a direction (nn_scan_forward.hip, nn_scan_backward.hip); `vectors`: every sequence's channels lie next
+// to each other. `room` holds room_for() bytes.
+void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, bool vectors, void *room);
+void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, bool vectors, void *room);
+// Bytes of workspace of either direction, whatever the operands' strides.
 int64_t room_for(const hmr_tensor_desc *gate);
 
 }  // namespace nn

@@ -1,0 +1,12 @@
+// The scan's kernels, backwards.
+#include "nn_scan.hpp"
+
+namespace hmr {
+namespace nn {
+
+void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, bool vectors, void *room) {
+    queue_scan<true>(stream, dtype, form, a, vectors, room);
+}
+
+}  // namespace nn
+}  // namespace hmr

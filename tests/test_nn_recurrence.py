@@ -178,6 +178,25 @@ def test_strided_sequences(layout, dtype):
         ref.assert_within(values(t), want[name], bounds[name], t.dtype, name)
 
 
+def test_steps_far_apart():
+    """Steps 3 million elements from each other, further than a scan's tile addresses."""
+    B, T, C, step = 2, 9, 40, 3_000_000
+    c = Case(DT.F32, B, T, C, True, 45)
+
+    def laid(v):
+        wide = np.zeros((T, step), np.float32)
+        wide[:, :B * C] = v.transpose(1, 0, 2).reshape(T, B * C)
+        return tensor(wide, DT.F32, [T, step], GPU).narrow(1, 0, B * C).as_strided([B, T, C], [C, step, 1], 0)
+
+    c.check_forward(laid(c.gate), laid(c.x))
+    state = ref.rounded(ref.recurrence(c.gate, c.x, c.initial, None, True, c.u)[0], DT.F32)
+    grad = ref.rounded(normal(9, c.x.size).reshape(c.x.shape), DT.F32)
+    got = h.grad_linear_recurrence(laid(grad), None, laid(c.gate), laid(c.x), laid(state), c.gpu_initial(), None, True)
+    want, bounds = ref.recurrence_backward(grad, None, c.gate, c.x, state, c.initial, None, True, c.u)
+    for name, t in zip(("d_gate", "d_input", "d_initial"), got):
+        ref.assert_within(values(t), want[name], bounds[name], t.dtype, name)
+
+
 @pytest.mark.parametrize("dtype", [DT.BF16, DT.F32], ids=lambda d: d.name)
 def test_a_gate_shared_by_a_head(dtype):
     """One gate per head, broadcast over its channels: its gradient is the sum over them."""
