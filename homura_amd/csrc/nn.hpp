@@ -76,18 +76,22 @@ struct Vec {
     static_assert(kBytes == 2 || kBytes % 4 == 0, "whole words, or one half");
     uint32_t w[kWords];
 
+    // NT: past the caches, for data that is used once and larger than they are.
+    template <bool NT = false>
     __device__ __forceinline__ void load(const T *p) {
         if constexpr (kBytes == 2) {
             w[0] = *reinterpret_cast<const uint16_t *>(p);
         } else {
 #pragma unroll
             for (int i = 0; i < kWords / kWide; ++i) {
-                const Access x = reinterpret_cast<const Access *>(p)[i];
+                const Access *q = reinterpret_cast<const Access *>(p) + i;
+                const Access x = NT ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
                 for (int k = 0; k < kWide; ++k) w[i * kWide + k] = x[k];
             }
         }
     }
+    template <bool NT = false>
     __device__ __forceinline__ void store(T *p) const {
         if constexpr (kBytes == 2) {
             *reinterpret_cast<uint16_t *>(p) = static_cast<uint16_t>(w[0]);
@@ -97,7 +101,9 @@ struct Vec {
                 Access x;
 #pragma unroll
                 for (int k = 0; k < kWide; ++k) x[k] = w[i * kWide + k];
-                reinterpret_cast<Access *>(p)[i] = x;
+                Access *q = reinterpret_cast<Access *>(p) + i;
+                if constexpr (NT) __builtin_nontemporal_store(x, q);
+                else *q = x;
             }
         }
     }
@@ -153,6 +159,21 @@ struct Vec {
         for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
     }
 };
+
+// How a kernel's large accesses treat the caches, fixed at compile time. A call that moves no more than the memory-side
+// cache holds leaves everything to the caches (the next call finds its input there); a larger one loads and stores past
+// them, but loads through them where rows begin inside cache lines, which neighbours then share.
+enum Passing : int { kThroughCaches = 0, kPastCaches = 1, kStoresPastCaches = 2 };
+
+inline Passing passing(int64_t bytes, bool whole_lines) {
+    return bytes <= kCacheResidentBytes ? kThroughCaches : (whole_lines ? kPastCaches : kStoresPastCaches);
+}
+
+// Calls f(IntTag<Passing>).
+template <class F>
+void with_passing(Passing p, F &&f) {
+    with_code(static_cast<int>(p), std::integer_sequence<int, kThroughCaches, kPastCaches, kStoresPastCaches>{}, f);
+}
 
 // One element of a tensor whose type is the computation type or, at run time, a narrower one.
 template <class T>

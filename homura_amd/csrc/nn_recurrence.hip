@@ -11,7 +11,6 @@ namespace {
 // that a tile of the scan spans more than its 32-bit offsets (2 million elements of 16 bits: time-major batches with as
 // many channels in all, which keep the memory busy a thread each). `last` may be
 // `initial`: a channel's state is read and written by its own thread.
-constexpr int64_t kFewSteps = 4;
 
 template <class T, int FORM>
 __global__ void __launch_bounds__(kBlock) forward_kernel(RecurrenceArgs a) {
@@ -106,12 +105,15 @@ RecurrenceArgs batch_args(const hmr_tensor_desc *gate, const hmr_tensor_desc *le
     return a;
 }
 
-// Whether every operand's channels lie next to each other.
-bool adjacent(std::initializer_list<const hmr_tensor_desc *> operands) {
+ScanLayout layout_of(std::initializer_list<const hmr_tensor_desc *> operands) {
+    ScanLayout layout{true, true};
     for (const hmr_tensor_desc *d : operands) {
-        if (d->strides[2] != 1) return false;
+        const int64_t size = dtype_size(d->dtype);
+        layout.adjacent = layout.adjacent && d->strides[2] == 1;
+        layout.whole_lines = layout.whole_lines && reinterpret_cast<uintptr_t>(first(*d)) % 128 == 0 && d->strides[0] * size % 128 == 0 &&
+                             d->strides[1] * size % 128 == 0;
     }
-    return true;
+    return layout;
 }
 
 // Whether a tile of the scan's largest shape spans less than 2^31 bytes in every operand.
@@ -144,8 +146,8 @@ hmr_status forward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *out, 
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
-            if (a.T > kFewSteps && near_by({gate, input, out})) {
-                queue_scan_forward(stream, gate->dtype, form, a, adjacent({gate, input, out}), workspace);
+            if (scan_used(gate) && near_by({gate, input, out})) {
+                queue_scan_forward(stream, gate->dtype, form, a, layout_of({gate, input, out}), workspace);
                 return;
             }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {
@@ -179,8 +181,8 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
-            if (a.T > kFewSteps && near_by({gate, input, out, grad, d_gate, d_input})) {
-                queue_scan_backward(stream, gate->dtype, form, a, adjacent({gate, input, out, grad, d_gate, d_input}), workspace);
+            if (scan_used(gate) && near_by({gate, input, out, grad, d_gate, d_input})) {
+                queue_scan_backward(stream, gate->dtype, form, a, layout_of({gate, input, out, grad, d_gate, d_input}), workspace);
                 return;
             }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {

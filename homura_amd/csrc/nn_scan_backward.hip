@@ -4,8 +4,8 @@
 namespace hmr {
 namespace nn {
 
-void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, bool vectors, void *room) {
-    queue_scan<true>(stream, dtype, form, a, vectors, room);
+void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, const ScanLayout &layout, void *room) {
+    queue_scan<true>(stream, dtype, form, a, layout, room);
 }
 
 }  // namespace nn

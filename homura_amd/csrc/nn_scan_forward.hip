@@ -4,19 +4,35 @@
 namespace hmr {
 namespace nn {
 
-void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, bool vectors, void *room) {
-    queue_scan<false>(stream, dtype, form, a, vectors, room);
+void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, const ScanLayout &layout, void *room) {
+    queue_scan<false>(stream, dtype, form, a, layout, room);
+}
+
+namespace {
+
+// The most that any shape makes of measure(shape, its plan).
+template <class F>
+int64_t most_of(const hmr_tensor_desc *gate, F measure) {
+    int64_t most = 0;
+    with_float_type(gate->dtype, [&](auto tag) {
+        with_scan_shapes<typename decltype(tag)::type>(gate->sizes[1], [&](auto shape) {
+            const int64_t x = measure(shape, decltype(shape)::plan(gate->sizes[1], gate->sizes[2]));
+            if (x > most) most = x;
+        });
+    });
+    return most;
+}
+
+}  // namespace
+
+bool scan_used(const hmr_tensor_desc *gate) {
+    return gate->sizes[1] > kFewSteps && gate->sizes[0] > 0 && gate->sizes[2] > 0 &&
+           most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }) <= kMostTiles;
 }
 
 int64_t room_for(const hmr_tensor_desc *gate) {
-    const int64_t B = gate->sizes[0], T = gate->sizes[1], C = gate->sizes[2];
-    if (B * C == 0) return 0;
-    switch (gate->dtype) {
-        case HMR_F16: return scan_room<f16_t>(B, T, C);
-        case HMR_BF16: return scan_room<bf16_t>(B, T, C);
-        case HMR_F32: return scan_room<float>(B, T, C);
-        default: return scan_room<double>(B, T, C);
-    }
+    if (!scan_used(gate)) return 0;
+    return 8 * most_of(gate, [&](auto shape, const ScanPlan &p) { return decltype(shape)::words(p, gate->sizes[0]); });
 }
 
 }  // namespace nn
