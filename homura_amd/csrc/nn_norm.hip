@@ -20,6 +20,9 @@ __device__ __forceinline__ double workgroup_sum(double v) {
 }
 
 // ---- one workgroup per group ---------------------------------------------------------------------------------
+//
+// Channels that do not lie next to each other, and short maps of huge groups: three passes over a group, element by
+// element.
 
 template <class T, int ACT>
 __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
@@ -145,7 +148,13 @@ NormArgs norm_args(const hmr_tensor_desc *src, int64_t groups) {
     return a;
 }
 
-int64_t norm_room(const hmr_tensor_desc *, int64_t, bool) { return 0; }
+// Workspace for whichever kernels the operands' strides will call for.
+int64_t norm_room(const hmr_tensor_desc *src, int64_t groups, bool backward) {
+    const NormArgs a = norm_args(src, groups);
+    if (a.C == 0) return 0;
+    const int64_t rows = norm_rows_room(a, src->dtype, backward), maps = norm_maps_room(a, src->dtype, backward);
+    return rows > maps ? rows : maps;
+}
 
 uint32_t grid_of(hmr_context_t ctx, int64_t groups) {
     const int64_t most = int64_t{64} * ctx->compute_units;
@@ -168,6 +177,8 @@ hmr_status forward(hmr_context_t ctx, const hmr_tensor_desc *out, const hmr_tens
     a.weight = per_channel(weight), a.bias = per_channel(bias), a.eps = eps;
     if (a.N == 0 || a.C == 0) return HMR_OK;
     return queue_on(ctx, who, [&](hipStream_t stream) {
+        if (queue_norm_rows(stream, src->dtype, a, activation, workspace, false)) return true;
+        if (queue_norm_maps(stream, src->dtype, a, activation, workspace, false)) return true;
         return with_float_type(src->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
             with_activation(activation, [&](auto act) {
@@ -194,6 +205,8 @@ hmr_status backward(hmr_context_t ctx, const hmr_tensor_desc *d_src, const hmr_t
     a.weight = per_channel(weight), a.bias = per_channel(bias), a.d_weight = per_channel(d_weight), a.d_bias = per_channel(d_bias);
     if (a.C == 0) return HMR_OK;
     return queue_on(ctx, who, [&](hipStream_t stream) {
+        if (queue_norm_rows(stream, src->dtype, a, activation, workspace, true)) return true;
+        if (queue_norm_maps(stream, src->dtype, a, activation, workspace, true)) return true;
         return with_float_type(src->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
             with_activation(activation, [&](auto act) {

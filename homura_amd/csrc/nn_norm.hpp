@@ -96,10 +96,135 @@ __device__ __forceinline__ typename Comp<T>::C bias_of(const PerChannel &b, int6
 
 // Calls f(IntTag<activation>) for a known activation.
 template <class F>
-bool with_activation(int32_t activation, F &&f) {
-    return with_code(activation, std::integer_sequence<int, HMN_ACTIVATION_NONE, HMR_UNARY_RELU, HMR_UNARY_SILU, HMR_UNARY_GELU,
-                                                       HMR_UNARY_GELU_TANH>{}, f);
+__host__ __device__ __forceinline__ bool with_activation(int32_t activation, F &&f) {
+    switch (activation) {
+        case HMN_ACTIVATION_NONE: f(IntTag<HMN_ACTIVATION_NONE>{}); return true;
+        case HMR_UNARY_RELU: f(IntTag<HMR_UNARY_RELU>{}); return true;
+        case HMR_UNARY_SILU: f(IntTag<HMR_UNARY_SILU>{}); return true;
+        case HMR_UNARY_GELU: f(IntTag<HMR_UNARY_GELU>{}); return true;
+        case HMR_UNARY_GELU_TANH: f(IntTag<HMR_UNARY_GELU_TANH>{}); return true;
+        default: return false;
+    }
 }
+// The same choice on the device, once for V elements (the activation is the launch's, so that nothing diverges).
+template <int V, class C>
+__device__ __forceinline__ void activate_all(int32_t activation, C (&z)[V]) {
+    with_activation(activation, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = activate<decltype(act)::value>(z[i]);
+    });
+}
+template <int V, class C>
+__device__ __forceinline__ void slope_all(int32_t activation, C (&z)[V]) {
+    with_activation(activation, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = slope<decltype(act)::value>(z[i]);
+    });
+}
+
+// ---- sums over lanes ------------------------------------------------------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return bits_as<float>(__builtin_amdgcn_update_dpp(0, bits_as<int>(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double v) {
+    const uint64_t b = bits_as<uint64_t>(v);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b)), CTRL, 0xF, 0xF, true));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b >> 32)), CTRL, 0xF, 0xF, true));
+    return bits_as<double>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+// The sum over each aligned run of `lanes` lanes (a power of two up to 64, the same for the whole wave), in every one of
+// them. Within 16 lanes neighbours meet through cross-lane moves of the vector unit: pairs, quads, then mirrored halves
+// (whose lanes agree by then), so that the order does not depend on the lane.
+template <class A>
+__device__ __forceinline__ A lanes_sum(A v, int lanes) {
+    if (lanes > 1) v += dpp_move<0xB1>(v);    // quad_perm [1, 0, 3, 2]
+    if (lanes > 2) v += dpp_move<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+    if (lanes > 4) v += dpp_move<0x141>(v);   // row_half_mirror
+    if (lanes > 8) v += dpp_move<0x140>(v);   // row_mirror
+    if (lanes > 16) v += __shfl_xor(v, 16, 64);
+    if (lanes > 32) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+// A mean as it is subtracted: in f32 as the nearest value and what is left, so that x - mean keeps its digits where x is
+// near a mean that is far from zero.
+template <class C>
+struct Centre;
+template <>
+struct Centre<float> {
+    float near, rest;
+    __device__ __forceinline__ explicit Centre(double mean) : near(static_cast<float>(mean)), rest(static_cast<float>(mean - static_cast<double>(near))) {}
+    __device__ __forceinline__ float from(float x) const { return (x - near) - rest; }
+};
+template <>
+struct Centre<double> {
+    double mean;
+    __device__ __forceinline__ explicit Centre(double m) : mean(m) {}
+    __device__ __forceinline__ double from(double x) const { return x - mean; }
+};
+
+// The weights or biases of V channels; `otherwise` without a tensor.
+template <class T, int V>
+__device__ __forceinline__ void load_channels(const PerChannel &w, int64_t c, typename Comp<T>::C otherwise, typename Comp<T>::C (&x)[V]) {
+    if (w.p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = otherwise;
+    } else if (w.sc == 1 && !w.wide) {
+        Vec<T, V> r;
+        r.load(reinterpret_cast<const T *>(w.p) + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = r.get(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = load_state<T>(w.p, (c + i) * w.sc, w.wide);
+    }
+}
+
+// ---- rows: a group in the registers of a wave or a workgroup ------------------------------------------------------------
+//
+// Where the elements of a group fit, one pass reads, reduces and writes them. A group's vectors (V channels each, so V
+// divides a group's channels) are spread over `lanes` lanes, M to a lane; a wave holds as many groups as fit side by side,
+// all of them in one row of channels where there are enough, else from several rows. Each lane keeps its channels from
+// row to row, so that the weights stay in registers (while they are few) and, backwards, the sums for the weights'
+// gradients do too: they leave the workgroup once, as a row of partial sums that a second launch adds up in order.
+struct RowsPlan {
+    int32_t v, m;         // vector width and vectors of a lane; m == 0: the groups do not fit
+    bool wide;            // a workgroup per group rather than lanes of a wave
+    int32_t lanes;        // of a group
+    int32_t vectors;      // of a group
+    int32_t per_position; // vectors of a group at one position
+    int32_t rows;         // of channels side by side in a wave
+    int64_t blocks;       // of groups, across a row
+    int64_t walkers;      // workgroups that share a block's rows
+};
+RowsPlan rows_plan(const NormArgs &a, int32_t dtype, bool backward);
+
+// ---- maps: groups spread over workgroups --------------------------------------------------------------------------------
+//
+// Larger groups take two passes over the maps, the second one out of the memory-side cache where they fit it. A
+// workgroup holds a run of positions (a chunk) of up to 256 vectors of channels: lane (r, l) walks every `slots`-th
+// position of its V channels. The first pass leaves each chunk's sums (per group forwards, per channel backwards), the
+// second one adds up what concerns it, in order, and writes.
+struct MapsPlan {
+    int32_t v;
+    int32_t lanes, slots;  // across channels and positions
+    int64_t blocks;        // of channels
+    int64_t chunks;        // of positions of one map
+    int64_t chunk;         // positions of one
+};
+MapsPlan maps_plan(const NormArgs &a, int32_t dtype);
+
+// Queue the kernels (nn_norm_rows.hip, nn_norm_maps.hip); false: the shape is not theirs.
+bool queue_norm_rows(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward);
+bool queue_norm_maps(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward);
+int64_t norm_rows_room(const NormArgs &a, int32_t dtype, bool backward);
+int64_t norm_maps_room(const NormArgs &a, int32_t dtype, bool backward);
+
+// Adds up `parts` rows of partial sums of C channels ([2][parts][C]: the weights', then the biases') into the gradients.
+void queue_weights_sum(hipStream_t stream, int32_t dtype, const NormArgs &a, const void *partial, int64_t parts);
 
 }  // namespace nn
 }  // namespace hmr

@@ -1,0 +1,427 @@
+// Group normalisation of groups that are spread over workgroups: chunks' sums, then the maps again.
+#include "nn_norm.hpp"
+
+namespace hmr {
+namespace nn {
+namespace {
+
+// What is known of a set of elements: in f64 the sum and the sum of squares, which keep the variance's digits for 16- and
+// 32-bit elements with means up to 2^12 deviations from zero; for F64 the mean and the squares about it, joined pairwise,
+// of the elements less the group's first one (a mean far from zero would take its digits from the joins' differences).
+template <class T>
+struct Moments {
+    double n, a, b;
+    __device__ __forceinline__ void add(const Moments &o) {
+        if constexpr (!std::is_same_v<T, double>) {
+            n += o.n, a += o.a, b += o.b;
+        } else if (o.n > 0) {
+            const double all = n + o.n, d = o.a - a;
+            a += d * (o.n / all);
+            b += o.b + d * d * (n * (o.n / all));
+            n = all;
+        }
+    }
+    __device__ __forceinline__ double mean(double less) const { return std::is_same_v<T, double> ? less + a : a / n; }
+    __device__ __forceinline__ double variance() const {
+        if constexpr (std::is_same_v<T, double>) return b / n;
+        const double m = a / n, v = __builtin_fma(-m, m, b / n);
+        return v < 0 ? 0 : v;
+    }
+};
+
+// What a group's elements are taken less.
+template <class T>
+__device__ __forceinline__ double less_of(const NormArgs &a, int64_t n, int64_t g) {
+    if constexpr (std::is_same_v<T, double>) return reinterpret_cast<const double *>(a.src.p)[n * a.src.sn + g * a.W];
+    else return 0;
+}
+
+struct MapsArgs {
+    NormArgs a;
+    MapsPlan p;
+    int32_t activation;
+    void *room;
+};
+
+// The workgroup's place: which map, which chunk of its positions, which block of channels; and the lane's.
+template <int V>
+struct Place {
+    int64_t n, chunk, block, s0, s1;  // positions of the chunk
+    int64_t c0, c1;                   // channels of the block
+    int slot;
+    int64_t c;  // the lane's first channel
+    bool on;
+    __device__ __forceinline__ Place(const NormArgs &a, const MapsPlan &p) {
+        block = blockIdx.x % p.blocks;
+        chunk = blockIdx.x / p.blocks % p.chunks, n = blockIdx.x / p.blocks / p.chunks;
+        s0 = chunk * p.chunk, s1 = s0 + p.chunk < a.S ? s0 + p.chunk : a.S;
+        c0 = block * p.lanes * V, c1 = c0 + p.lanes * V < a.C ? c0 + p.lanes * V : a.C;
+        slot = threadIdx.x / p.lanes;
+        c = c0 + threadIdx.x % p.lanes * V;
+        on = slot < p.slots && c < a.C;
+    }
+};
+
+constexpr int kAtOnce = 4;  // positions of a lane in flight
+
+// Calls f(vector) for the lane's vectors of `x`, kAtOnce loads at a time.
+template <class T, int V, class F>
+__device__ __forceinline__ void for_positions(const Place<V> &at, const MapsPlan &p, const Maps &x, F f) {
+    if (!at.on) return;
+    const T *from = reinterpret_cast<const T *>(x.p) + at.n * x.sn + at.c;
+    for (int64_t s = at.s0 + at.slot; s < at.s1; s += kAtOnce * p.slots) {
+        Vec<T, V> v[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (s + k * p.slots < at.s1) v[k].load(from + (s + k * p.slots) * x.ss);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (s + k * p.slots < at.s1) f(s + k * p.slots, v[k]);
+        }
+    }
+}
+template <class T, int V, class F>
+__device__ __forceinline__ void for_positions(const Place<V> &at, const MapsPlan &p, const Maps &x, const Maps &y, F f) {
+    if (!at.on) return;
+    const T *from = reinterpret_cast<const T *>(x.p) + at.n * x.sn + at.c, *from_y = reinterpret_cast<const T *>(y.p) + at.n * y.sn + at.c;
+    for (int64_t s = at.s0 + at.slot; s < at.s1; s += kAtOnce * p.slots) {
+        Vec<T, V> v[kAtOnce], w[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (s + k * p.slots < at.s1) v[k].load(from + (s + k * p.slots) * x.ss), w[k].load(from_y + (s + k * p.slots) * y.ss);
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (s + k * p.slots < at.s1) f(s + k * p.slots, v[k], w[k]);
+        }
+    }
+}
+
+// ---- forwards ---------------------------------------------------------------------------------------------------------
+
+// [N][chunks][blocks][G] moments; a block writes those of the groups it has channels of.
+template <class T, int V>
+__global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
+    const NormArgs &a = m.a;
+    const Place<V> at(a, m.p);
+    // Of each of the lane's channels. F64 sums about the first one that the lane meets.
+    double n = 0, sum[V], squares[V], about[V], less[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        sum[i] = squares[i] = about[i] = 0;
+        less[i] = at.on ? less_of<T>(a, at.n, (at.c + i) / a.W) : 0;
+    }
+    for_positions<T, V>(at, m.p, a.src, [&](int64_t, const Vec<T, V> &x) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            double v = x.get(i);
+            if constexpr (std::is_same_v<T, double>) {
+                v -= less[i];
+                if (n == 0) about[i] = v;
+                v -= about[i];
+            }
+            sum[i] += v, squares[i] = __builtin_fma(v, v, squares[i]);
+        }
+        n += 1;
+    });
+    __shared__ double slots_sum[kBlock][V], slots_squares[kBlock][V], slots_n[kBlock];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (std::is_same_v<T, double>) {
+            const double shift = n > 0 ? sum[i] / n : 0;
+            slots_sum[threadIdx.x][i] = about[i] + shift;
+            slots_squares[threadIdx.x][i] = squares[i] - shift * sum[i];
+        } else {
+            slots_sum[threadIdx.x][i] = sum[i], slots_squares[threadIdx.x][i] = squares[i];
+        }
+    }
+    slots_n[threadIdx.x] = n;
+    __syncthreads();
+    // The slots of a channel, in order, by the first slot's lanes.
+    if (at.on && at.slot == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            Moments<T> all{slots_n[threadIdx.x], slots_sum[threadIdx.x][i], slots_squares[threadIdx.x][i]};
+            for (int k = 1; k < m.p.slots; ++k) {
+                const int l = threadIdx.x + k * m.p.lanes;
+                all.add(Moments<T>{slots_n[l], slots_sum[l][i], slots_squares[l][i]});
+            }
+            slots_sum[threadIdx.x][i] = all.a, slots_squares[threadIdx.x][i] = all.b;
+        }
+    }
+    __syncthreads();
+    const double positions = static_cast<double>(at.s1 - at.s0);
+    Moments<T> *out = static_cast<Moments<T> *>(m.room) + ((at.n * m.p.chunks + at.chunk) * m.p.blocks + at.block) * a.G;
+    for (int64_t g = at.c0 / a.W + threadIdx.x; g * a.W < at.c1; g += kBlock) {
+        const int64_t from = g * a.W > at.c0 ? g * a.W : at.c0, to = (g + 1) * a.W < at.c1 ? (g + 1) * a.W : at.c1;
+        Moments<T> all{0, 0, 0};
+        for (int64_t c = from - at.c0; c < to - at.c0; ++c) all.add(Moments<T>{positions, slots_sum[c / V][c % V], slots_squares[c / V][c % V]});
+        out[g] = all;
+    }
+}
+
+// The moments of group g of map n, by `lanes` neighbouring threads of which this is `lane`, a power of two up to 64; in
+// every one of them the same.
+template <class T>
+__device__ __forceinline__ Moments<T> gather(const MapsArgs &m, int64_t n, int64_t g, int64_t block_channels, int lane, int lanes, bool on) {
+    const NormArgs &a = m.a;
+    const int64_t first = g * a.W / block_channels, last = ((g + 1) * a.W - 1) / block_channels, across = last - first + 1;
+    const Moments<T> *in = static_cast<const Moments<T> *>(m.room) + n * m.p.chunks * m.p.blocks * a.G + g;
+    Moments<T> all{0, 0, 0};
+    if (on) {
+        for (int64_t k = lane; k < m.p.chunks * across; k += lanes) all.add(in[(k / across * m.p.blocks + first + k % across) * a.G]);
+    }
+    for (int d = 1; d < lanes; d <<= 1) {
+        Moments<T> other{__shfl_xor(all.n, d, 64), __shfl_xor(all.a, d, 64), __shfl_xor(all.b, d, 64)};
+        // Joined lower lane first on both sides, so that they agree.
+        if (lane & d) {
+            Moments<T> low = other;
+            low.add(all);
+            all = low;
+        } else {
+            all.add(other);
+        }
+    }
+    return all;
+}
+
+template <class T, int V, bool PAST>
+__global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
+    using C = typename Comp<T>::C;
+    const NormArgs &a = m.a;
+    const Place<V> at(a, m.p);
+    // The block's groups' means and reciprocal deviations.
+    extern __shared__ double statistics[];  // [2][groups of the block]
+    const int64_t g0 = at.c0 / a.W, groups = (at.c1 - 1) / a.W - g0 + 1, room = (m.p.lanes * V - 1) / a.W + 2;
+    int lanes = 64;
+    while (lanes > 1 && kBlock / lanes < groups) lanes /= 2;
+    const int each = kBlock / lanes;
+    for (int64_t k0 = 0; k0 < groups; k0 += each) {
+        const int64_t k = k0 + threadIdx.x / lanes;
+        const Moments<T> all = gather<T>(m, at.n, k < groups ? g0 + k : g0, static_cast<int64_t>(m.p.lanes) * V, threadIdx.x % lanes, lanes, k < groups);
+        if (k < groups && threadIdx.x % lanes == 0) {
+            const double mean = all.mean(less_of<T>(a, at.n, g0 + k)), rstd = 1.0 / sqrt(all.variance() + a.eps);
+            statistics[k] = mean, statistics[room + k] = rstd;
+            // One workgroup of the map writes a group's statistics: the first chunk's, in the block where the group begins.
+            if (at.chunk == 0 && (g0 + k) * a.W >= at.c0) {
+                if (a.mean.p != nullptr) reinterpret_cast<C *>(a.mean.p)[a.mean.at(at.n, g0 + k)] = static_cast<C>(mean);
+                if (a.rstd.p != nullptr) reinterpret_cast<C *>(a.rstd.p)[a.rstd.at(at.n, g0 + k)] = static_cast<C>(rstd);
+            }
+        }
+    }
+    __syncthreads();
+    if (!at.on) return;
+    C w[V], b[V], rstd[V];
+    load_channels<T, V>(a.weight, at.c, C(1), w);
+    load_channels<T, V>(a.bias, at.c, C(0), b);
+    double mean[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int64_t k = (at.c + i) / a.W - g0;
+        mean[i] = statistics[k], rstd[i] = static_cast<C>(statistics[room + k]);
+    }
+    T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
+    for_positions<T, V>(at, m.p, a.src, [&](int64_t s, const Vec<T, V> &x) {
+        C z[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = Centre<C>(mean[i]).from(x.get(i)) * rstd[i] * w[i] + b[i];
+        activate_all<V>(m.activation, z);
+        Vec<T, V> y;
+        y.round(z);
+        y.template store<PAST>(to + s * a.out.ss);
+    });
+}
+
+// ---- backwards --------------------------------------------------------------------------------------------------------
+
+// hat, and in z the derivative of what it leads to.
+template <class T, int V, class C>
+__device__ __forceinline__ void hat_and_slope(int32_t activation, const Vec<T, V> &x, const C (&mean)[V], const C (&rstd)[V], const C (&w)[V],
+                                              const C (&b)[V], C (&hat)[V], C (&z)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        hat[i] = (x.get(i) - mean[i]) * rstd[i];
+        z[i] = hat[i] * w[i] + b[i];
+    }
+    slope_all<V>(activation, z);
+}
+template <class T, int V, class C>
+__device__ __forceinline__ void load_statistics(const NormArgs &a, int64_t n, int64_t c, C (&mean)[V], C (&rstd)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int64_t g = (c + i) / a.W;
+        mean[i] = reinterpret_cast<const C *>(a.mean.p)[a.mean.at(n, g)], rstd[i] = reinterpret_cast<const C *>(a.rstd.p)[a.rstd.at(n, g)];
+    }
+}
+
+// Rows of sums per channel, [2][N * chunks][C]: of d * hat, and of d.
+template <class T, int V>
+__global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
+    using C = typename Comp<T>::C;
+    const NormArgs &a = m.a;
+    const Place<V> at(a, m.p);
+    C sum[V], sum_h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = sum_h[i] = 0;
+    if (at.on) {
+        C w[V], b[V], mean[V], rstd[V];
+        load_channels<T, V>(a.weight, at.c, C(1), w);
+        load_channels<T, V>(a.bias, at.c, C(0), b);
+        load_statistics<T, V>(a, at.n, at.c, mean, rstd);
+        for_positions<T, V>(at, m.p, a.src, a.grad, [&](int64_t, const Vec<T, V> &x, const Vec<T, V> &dy) {
+            C hat[V], z[V];
+            hat_and_slope<T, V>(m.activation, x, mean, rstd, w, b, hat, z);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const C d = dy.get(i) * z[i];
+                sum[i] += d, sum_h[i] += d * hat[i];
+            }
+        });
+    }
+    __shared__ C slots[2][kBlock][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) slots[0][threadIdx.x][i] = sum_h[i], slots[1][threadIdx.x][i] = sum[i];
+    __syncthreads();
+    if (at.on && at.slot == 0) {
+        C *out = static_cast<C *>(m.room);
+        const int64_t parts = a.N * m.p.chunks, part = at.n * m.p.chunks + at.chunk;
+        for (int which = 0; which < 2; ++which) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                double total = 0;
+                for (int k = 0; k < m.p.slots; ++k) total += slots[which][threadIdx.x + k * m.p.lanes][i];
+                out[(which * parts + part) * a.C + at.c + i] = static_cast<C>(total);
+            }
+        }
+    }
+}
+
+// The means over each group, [N * G][2] of f64 behind the rows: of weight * d, and of weight * d * hat. A workgroup a group.
+template <class T>
+__global__ void __launch_bounds__(kBlock) group_means_kernel(MapsArgs m, double *means) {
+    using C = typename Comp<T>::C;
+    const NormArgs &a = m.a;
+    const int64_t n = blockIdx.x / a.G, g = blockIdx.x % a.G, parts = a.N * m.p.chunks;
+    const C *in = static_cast<const C *>(m.room);
+    double sum = 0, sum_h = 0;
+    for (int64_t k = threadIdx.x; k < m.p.chunks * a.W; k += kBlock) {
+        const int64_t part = n * m.p.chunks + k / a.W, c = g * a.W + k % a.W;
+        const double w = weight_of<T>(a.weight, c);
+        sum_h += w * in[part * a.C + c], sum += w * in[(parts + part) * a.C + c];
+    }
+    sum = lanes_sum(sum, 64), sum_h = lanes_sum(sum_h, 64);
+    __shared__ double waves[2][kBlock / 64];
+    if (threadIdx.x % 64 == 0) waves[0][threadIdx.x / 64] = sum, waves[1][threadIdx.x / 64] = sum_h;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        double total = 0;
+#pragma unroll
+        for (int k = 0; k < kBlock / 64; ++k) total += waves[threadIdx.x][k];
+        means[2 * blockIdx.x + threadIdx.x] = total / (static_cast<double>(a.S) * static_cast<double>(a.W));
+    }
+}
+
+template <class T, int V, bool PAST>
+__global__ void __launch_bounds__(kBlock) apply_back_kernel(MapsArgs m, const double *means) {
+    using C = typename Comp<T>::C;
+    const NormArgs &a = m.a;
+    const Place<V> at(a, m.p);
+    if (!at.on) return;
+    C w[V], b[V], mean[V], rstd[V], d_mean[V], dh_mean[V];
+    load_channels<T, V>(a.weight, at.c, C(1), w);
+    load_channels<T, V>(a.bias, at.c, C(0), b);
+    load_statistics<T, V>(a, at.n, at.c, mean, rstd);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const double *p = means + 2 * (at.n * a.G + (at.c + i) / a.W);
+        d_mean[i] = static_cast<C>(p[0]), dh_mean[i] = static_cast<C>(p[1]);
+    }
+    T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
+    for_positions<T, V>(at, m.p, a.src, a.grad, [&](int64_t s, const Vec<T, V> &x, const Vec<T, V> &dy) {
+        C hat[V], z[V];
+        hat_and_slope<T, V>(m.activation, x, mean, rstd, w, b, hat, z);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = rstd[i] * (w[i] * (dy.get(i) * z[i]) - d_mean[i] - hat[i] * dh_mean[i]);
+        Vec<T, V> dx;
+        dx.round(z);
+        dx.template store<PAST>(to + s * a.out.ss);
+    });
+}
+
+int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+int64_t rows_bytes(const NormArgs &a, const MapsPlan &p, int32_t dtype) {
+    return up16(2 * a.N * p.chunks * a.C * dtype_size(wide_type(dtype)));
+}
+
+template <class T, int V>
+void launch_maps(hipStream_t stream, const MapsArgs &m, bool backward, bool past) {
+    const NormArgs &a = m.a;
+    const uint32_t groups = static_cast<uint32_t>(a.N * m.p.chunks * m.p.blocks);
+    if (!backward) {
+        moments_kernel<T, V><<<groups, kBlock, 0, stream>>>(m);
+        const size_t lds = 2 * sizeof(double) * static_cast<size_t>((m.p.lanes * V - 1) / a.W + 2);
+        if (past) apply_kernel<T, V, true><<<groups, kBlock, lds, stream>>>(m);
+        else apply_kernel<T, V, false><<<groups, kBlock, lds, stream>>>(m);
+        return;
+    }
+    double *means = reinterpret_cast<double *>(static_cast<char *>(m.room) + rows_bytes(a, m.p, sizeof(T) == 2 ? HMR_BF16 : (sizeof(T) == 4 ? HMR_F32 : HMR_F64)));
+    channel_sums_kernel<T, V><<<groups, kBlock, 0, stream>>>(m);
+    group_means_kernel<T><<<static_cast<uint32_t>(a.N * a.G), kBlock, 0, stream>>>(m, means);
+    if (past) apply_back_kernel<T, V, true><<<groups, kBlock, 0, stream>>>(m, means);
+    else apply_back_kernel<T, V, false><<<groups, kBlock, 0, stream>>>(m, means);
+}
+
+}  // namespace
+
+MapsPlan maps_plan(const NormArgs &a, int32_t dtype) {
+    MapsPlan p{};
+    const int full = 16 / dtype_size(dtype);
+    p.v = a.C % full == 0 ? full : (full == 8 && a.C % 2 == 0 ? 2 : 1);
+    const int64_t across = a.C / p.v;
+    p.lanes = static_cast<int32_t>(across < kBlock ? across : kBlock);
+    p.slots = kBlock / p.lanes;
+    p.blocks = (across + p.lanes - 1) / p.lanes;
+    // Eight workgroups for every compute unit, but no chunk shorter than what a workgroup requests at once.
+    const int64_t shortest = kAtOnce * p.slots, most = (a.S + shortest - 1) / shortest;
+    int64_t chunks = (2048 + a.N * p.blocks - 1) / (a.N * p.blocks);
+    chunks = chunks < 1 ? 1 : (chunks > most ? most : chunks);
+    p.chunk = (a.S + chunks - 1) / chunks;
+    p.chunks = (a.S + p.chunk - 1) / p.chunk;
+    return p;
+}
+
+namespace {
+// Short maps of huge groups would leave rows of sums as large as themselves; so many workgroups do not make a launch.
+bool maps_fit(const NormArgs &a, int32_t dtype) {
+    if (a.N == 0 || a.S == 0 || a.C == 0) return false;
+    if (a.S < 8 && a.N * a.C > (int64_t{1} << 22)) return false;
+    const MapsPlan p = maps_plan(a, dtype);
+    return a.N * p.chunks * p.blocks < (int64_t{1} << 31) && a.N * a.G < (int64_t{1} << 31);
+}
+}  // namespace
+
+int64_t norm_maps_room(const NormArgs &a, int32_t dtype, bool backward) {
+    if (!maps_fit(a, dtype)) return 0;
+    const MapsPlan p = maps_plan(a, dtype);
+    if (!backward) return a.N * p.chunks * p.blocks * a.G * static_cast<int64_t>(3 * sizeof(double));
+    return rows_bytes(a, p, dtype) + a.N * a.G * static_cast<int64_t>(2 * sizeof(double));
+}
+
+bool queue_norm_maps(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward) {
+    if (a.src.sc != 1 || a.out.sc != 1 || (backward && a.grad.sc != 1) || !maps_fit(a, dtype)) return false;
+    MapsArgs m{a, maps_plan(a, dtype), activation, room};
+    const bool past = a.N * a.S * a.C * dtype_size(dtype) * (backward ? 3 : 2) > kCacheResidentBytes;
+    with_float_type(dtype, [&](auto tag) {
+        using T = typename decltype(tag)::type;
+        constexpr int kFull = 16 / static_cast<int>(sizeof(T));
+        if (m.p.v == kFull) launch_maps<T, kFull>(stream, m, backward, past);
+        else if (kFull == 8 && m.p.v == 2) launch_maps<T, kFull == 8 ? 2 : 1>(stream, m, backward, past);
+        else launch_maps<T, 1>(stream, m, backward, past);
+    });
+    if (backward && (a.d_weight.p != nullptr || a.d_bias.p != nullptr)) queue_weights_sum(stream, dtype, a, room, a.N * m.p.chunks);
+    return true;
+}
+
+}  // namespace nn
+}  // namespace hmr
