@@ -64,6 +64,9 @@ inline hmr_status check_room(const char *who, const void *workspace, int64_t hav
 
 // ---- device side --------------------------------------------------------------------------------------------------
 
+__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
 // V elements of type T as memory holds them, moved in accesses of up to 16 bytes. The vectors need no more alignment than
 // an element has (global accesses of this target take any), so a row of odd length or an odd start costs a few split
 // lines, not another kernel.

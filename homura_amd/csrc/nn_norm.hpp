@@ -56,12 +56,17 @@ constexpr double kRootTwoByPi = 0.79788456080286535588;    // sqrt(2/pi)
 constexpr double kTanhInner = 0.044715;
 
 // (1 + tanh(u)) / 2 is the logistic function of 2 u, which keeps its digits where tanh nears -1.
+template <class C>
+__device__ __forceinline__ C tanh_gate(C z) {
+    return logistic(z * fma_(C(2 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)));
+}
+
 template <int ACT, class C>
 __device__ __forceinline__ C activate(C z) {
     if constexpr (ACT == HMR_UNARY_RELU) return z < C(0) ? C(0) : z;
     else if constexpr (ACT == HMR_UNARY_SILU) return z * logistic(z);
     else if constexpr (ACT == HMR_UNARY_GELU) return C(0.5) * z * erfc(-z * C(kRootHalf));
-    else if constexpr (ACT == HMR_UNARY_GELU_TANH) return z * logistic(C(2 * kRootTwoByPi) * (z + C(kTanhInner) * z * z * z));
+    else if constexpr (ACT == HMR_UNARY_GELU_TANH) return z * tanh_gate(z);
     else return z;
 }
 
@@ -71,12 +76,12 @@ __device__ __forceinline__ C slope(C z) {
         return z > C(0) ? C(1) : (z != z ? z : C(0));
     } else if constexpr (ACT == HMR_UNARY_SILU) {
         const C q = logistic(z);
-        return q * (C(1) + z * (C(1) - q));
+        return fma_(z * q, C(1) - q, q);
     } else if constexpr (ACT == HMR_UNARY_GELU) {
         return C(0.5) * erfc(-z * C(kRootHalf)) + z * exp(C(-0.5) * z * z) * C(0.5 * kRootTwoByPi);
     } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
-        const C q = logistic(C(2 * kRootTwoByPi) * (z + C(kTanhInner) * z * z * z));
-        return q * (C(1) + z * (C(1) - q) * C(2 * kRootTwoByPi) * (C(1) + C(3 * kTanhInner) * z * z));
+        const C q = tanh_gate(z);
+        return fma_(z * q * (C(1) - q), fma_(C(6 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)), q);
     } else {
         return C(1);
     }
@@ -111,14 +116,22 @@ template <int V, class C>
 __device__ __forceinline__ void activate_all(int32_t activation, C (&z)[V]) {
     with_activation(activation, [&](auto act) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate<decltype(act)::value>(z[i]);
+        for (int i = 0; i < V; ++i) {
+            z[i] = activate<decltype(act)::value>(z[i]);
+            // The error function's many intermediate values, of one element at a time.
+            if constexpr (decltype(act)::value == HMR_UNARY_GELU) __builtin_amdgcn_sched_barrier(0);
+        }
     });
 }
 template <int V, class C>
 __device__ __forceinline__ void slope_all(int32_t activation, C (&z)[V]) {
     with_activation(activation, [&](auto act) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = slope<decltype(act)::value>(z[i]);
+        for (int i = 0; i < V; ++i) {
+            z[i] = slope<decltype(act)::value>(z[i]);
+            // The error function's many intermediate values, of one element at a time.
+            if constexpr (decltype(act)::value == HMR_UNARY_GELU) __builtin_amdgcn_sched_barrier(0);
+        }
     });
 }
 
@@ -156,31 +169,41 @@ struct Centre;
 template <>
 struct Centre<float> {
     float near, rest;
+    Centre() = default;
     __device__ __forceinline__ explicit Centre(double mean) : near(static_cast<float>(mean)), rest(static_cast<float>(mean - static_cast<double>(near))) {}
     __device__ __forceinline__ float from(float x) const { return (x - near) - rest; }
 };
 template <>
 struct Centre<double> {
     double mean;
+    Centre() = default;
     __device__ __forceinline__ explicit Centre(double m) : mean(m) {}
     __device__ __forceinline__ double from(double x) const { return x - mean; }
 };
 
-// The weights or biases of V channels; `otherwise` without a tensor.
+// The weights or biases of V channels, which lie next to each other; `otherwise` without a tensor.
 template <class T, int V>
 __device__ __forceinline__ void load_channels(const PerChannel &w, int64_t c, typename Comp<T>::C otherwise, typename Comp<T>::C (&x)[V]) {
     if (w.p == nullptr) {
 #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = otherwise;
-    } else if (w.sc == 1 && !w.wide) {
+    } else if (!w.wide) {
         Vec<T, V> r;
         r.load(reinterpret_cast<const T *>(w.p) + c);
 #pragma unroll
         for (int i = 0; i < V; ++i) x[i] = r.get(i);
     } else {
+        Vec<typename Comp<T>::C, V> r;
+        r.load(reinterpret_cast<const typename Comp<T>::C *>(w.p) + c);
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = load_state<T>(w.p, (c + i) * w.sc, w.wide);
+        for (int i = 0; i < V; ++i) x[i] = r.get(i);
     }
+}
+
+// Whether the fast kernels take the operands: everything that has channels has them next to each other.
+inline bool channels_adjacent(const NormArgs &a, bool backward) {
+    auto dense = [](const PerChannel &w) { return w.p == nullptr || w.sc == 1; };
+    return a.src.sc == 1 && a.out.sc == 1 && (!backward || a.grad.sc == 1) && dense(a.weight) && dense(a.bias);
 }
 
 // ---- rows: a group in the registers of a wave or a workgroup ------------------------------------------------------------

@@ -62,41 +62,54 @@ struct Place {
     }
 };
 
-constexpr int kAtOnce = 4;  // positions of a lane in flight
+constexpr int kAtOnce = 4;  // positions of a lane requested at a time
 
-// Calls f(vector) for the lane's vectors of `x`, kAtOnce loads at a time.
-template <class T, int V, class F>
-__device__ __forceinline__ void for_positions(const Place<V> &at, const MapsPlan &p, const Maps &x, F f) {
-    if (!at.on) return;
-    const T *from = reinterpret_cast<const T *>(x.p) + at.n * x.sn + at.c;
-    for (int64_t s = at.s0 + at.slot; s < at.s1; s += kAtOnce * p.slots) {
-        Vec<T, V> v[kAtOnce];
+// A lane's walk through its positions of one or two maps: the next vectors are under way while f works on these, the first
+// ones from the walk's beginning on.
+template <class T, int V, int MAPS>
+struct Walk {
+    const T *from[MAPS];
+    int64_t step[MAPS], s, s1;  // between positions; the next position, the chunk's end
+    int slots;
+    Vec<T, V> next[MAPS][kAtOnce];
+
+    __device__ __forceinline__ Walk(const Place<V> &at, const MapsPlan &p, const Maps &x, const Maps &y)
+        : s(at.s0 + at.slot), s1(at.on ? at.s1 : 0), slots(p.slots) {
+        from[0] = reinterpret_cast<const T *>(x.p) + at.n * x.sn + at.c, step[0] = x.ss;
+        if constexpr (MAPS == 2) from[1] = reinterpret_cast<const T *>(y.p) + at.n * y.sn + at.c, step[1] = y.ss;
+        fetch();
+    }
+    __device__ __forceinline__ void fetch() {
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            if (s + k * p.slots < at.s1) v[k].load(from + (s + k * p.slots) * x.ss);
-        }
+            if (s + k * slots < s1) {
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            if (s + k * p.slots < at.s1) f(s + k * p.slots, v[k]);
+                for (int j = 0; j < MAPS; ++j) next[j][k].load(from[j] + (s + k * slots) * step[j]);
+            }
         }
     }
-}
-template <class T, int V, class F>
-__device__ __forceinline__ void for_positions(const Place<V> &at, const MapsPlan &p, const Maps &x, const Maps &y, F f) {
-    if (!at.on) return;
-    const T *from = reinterpret_cast<const T *>(x.p) + at.n * x.sn + at.c, *from_y = reinterpret_cast<const T *>(y.p) + at.n * y.sn + at.c;
-    for (int64_t s = at.s0 + at.slot; s < at.s1; s += kAtOnce * p.slots) {
-        Vec<T, V> v[kAtOnce], w[kAtOnce];
+    template <class F>
+    __device__ __forceinline__ void run(F f) {
+        while (s < s1) {
+            Vec<T, V> now[MAPS][kAtOnce];
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            if (s + k * p.slots < at.s1) v[k].load(from + (s + k * p.slots) * x.ss), w[k].load(from_y + (s + k * p.slots) * y.ss);
-        }
+            for (int j = 0; j < MAPS; ++j) {
 #pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-            if (s + k * p.slots < at.s1) f(s + k * p.slots, v[k], w[k]);
+                for (int k = 0; k < kAtOnce; ++k) now[j][k] = next[j][k];
+            }
+            const int64_t here = s;
+            s += kAtOnce * slots;
+            fetch();
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                if (here + k * slots < s1) {
+                    if constexpr (MAPS == 2) f(here + k * slots, now[0][k], now[1][k]);
+                    else f(here + k * slots, now[0][k]);
+                }
+            }
         }
     }
-}
+};
 
 // ---- forwards ---------------------------------------------------------------------------------------------------------
 
@@ -105,6 +118,7 @@ template <class T, int V>
 __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
+    Walk<T, V, 1> walk(at, m.p, a.src, a.src);
     // Of each of the lane's channels. F64 sums about the first one that the lane meets.
     double n = 0, sum[V], squares[V], about[V], less[V];
 #pragma unroll
@@ -112,7 +126,7 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
         sum[i] = squares[i] = about[i] = 0;
         less[i] = at.on ? less_of<T>(a, at.n, (at.c + i) / a.W) : 0;
     }
-    for_positions<T, V>(at, m.p, a.src, [&](int64_t, const Vec<T, V> &x) {
+    walk.run([&](int64_t, const Vec<T, V> &x) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             double v = x.get(i);
@@ -166,11 +180,24 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
 template <class T>
 __device__ __forceinline__ Moments<T> gather(const MapsArgs &m, int64_t n, int64_t g, int64_t block_channels, int lane, int lanes, bool on) {
     const NormArgs &a = m.a;
-    const int64_t first = g * a.W / block_channels, last = ((g + 1) * a.W - 1) / block_channels, across = last - first + 1;
+    const int64_t first = g * a.W / block_channels, last = ((g + 1) * a.W - 1) / block_channels;
     const Moments<T> *in = static_cast<const Moments<T> *>(m.room) + n * m.p.chunks * m.p.blocks * a.G + g;
     Moments<T> all{0, 0, 0};
     if (on) {
-        for (int64_t k = lane; k < m.p.chunks * across; k += lanes) all.add(in[(k / across * m.p.blocks + first + k % across) * a.G]);
+        constexpr int kAhead = 4;  // loads in flight
+        for (int64_t b = first; b <= last; ++b) {
+            for (int64_t k = lane; k < m.p.chunks; k += kAhead * lanes) {
+                Moments<T> some[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (k + j * lanes < m.p.chunks) some[j] = in[((k + j * lanes) * m.p.blocks + b) * a.G];
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (k + j * lanes < m.p.chunks) all.add(some[j]);
+                }
+            }
+        }
     }
     for (int d = 1; d < lanes; d <<= 1) {
         Moments<T> other{__shfl_xor(all.n, d, 64), __shfl_xor(all.a, d, 64), __shfl_xor(all.b, d, 64)};
@@ -191,6 +218,10 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
     using C = typename Comp<T>::C;
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
+    Walk<T, V, 1> walk(at, m.p, a.src, a.src);
+    C w[V], b[V], rstd[V];
+    load_channels<T, V>(a.weight, at.on ? at.c : 0, C(1), w);
+    load_channels<T, V>(a.bias, at.on ? at.c : 0, C(0), b);
     // The block's groups' means and reciprocal deviations.
     extern __shared__ double statistics[];  // [2][groups of the block]
     const int64_t g0 = at.c0 / a.W, groups = (at.c1 - 1) / a.W - g0 + 1, room = (m.p.lanes * V - 1) / a.W + 2;
@@ -212,20 +243,17 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
     }
     __syncthreads();
     if (!at.on) return;
-    C w[V], b[V], rstd[V];
-    load_channels<T, V>(a.weight, at.c, C(1), w);
-    load_channels<T, V>(a.bias, at.c, C(0), b);
-    double mean[V];
+    Centre<C> centre[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int64_t k = (at.c + i) / a.W - g0;
-        mean[i] = statistics[k], rstd[i] = static_cast<C>(statistics[room + k]);
+        centre[i] = Centre<C>(statistics[k]), rstd[i] = static_cast<C>(statistics[room + k]);
     }
     T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
-    for_positions<T, V>(at, m.p, a.src, [&](int64_t s, const Vec<T, V> &x) {
+    walk.run([&](int64_t s, const Vec<T, V> &x) {
         C z[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = Centre<C>(mean[i]).from(x.get(i)) * rstd[i] * w[i] + b[i];
+        for (int i = 0; i < V; ++i) z[i] = fma_(centre[i].from(x.get(i)) * rstd[i], w[i], b[i]);
         activate_all<V>(m.activation, z);
         Vec<T, V> y;
         y.round(z);
@@ -242,7 +270,7 @@ __device__ __forceinline__ void hat_and_slope(int32_t activation, const Vec<T, V
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         hat[i] = (x.get(i) - mean[i]) * rstd[i];
-        z[i] = hat[i] * w[i] + b[i];
+        z[i] = fma_(hat[i], w[i], b[i]);
     }
     slope_all<V>(activation, z);
 }
@@ -261,6 +289,7 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
     using C = typename Comp<T>::C;
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
+    Walk<T, V, 2> walk(at, m.p, a.src, a.grad);
     C sum[V], sum_h[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = sum_h[i] = 0;
@@ -269,13 +298,13 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
         load_channels<T, V>(a.weight, at.c, C(1), w);
         load_channels<T, V>(a.bias, at.c, C(0), b);
         load_statistics<T, V>(a, at.n, at.c, mean, rstd);
-        for_positions<T, V>(at, m.p, a.src, a.grad, [&](int64_t, const Vec<T, V> &x, const Vec<T, V> &dy) {
+        walk.run([&](int64_t, const Vec<T, V> &x, const Vec<T, V> &dy) {
             C hat[V], z[V];
             hat_and_slope<T, V>(m.activation, x, mean, rstd, w, b, hat, z);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const C d = dy.get(i) * z[i];
-                sum[i] += d, sum_h[i] += d * hat[i];
+                sum[i] += d, sum_h[i] = fma_(d, hat[i], sum_h[i]);
             }
         });
     }
@@ -305,10 +334,24 @@ __global__ void __launch_bounds__(kBlock) group_means_kernel(MapsArgs m, double 
     const int64_t n = blockIdx.x / a.G, g = blockIdx.x % a.G, parts = a.N * m.p.chunks;
     const C *in = static_cast<const C *>(m.room);
     double sum = 0, sum_h = 0;
-    for (int64_t k = threadIdx.x; k < m.p.chunks * a.W; k += kBlock) {
-        const int64_t part = n * m.p.chunks + k / a.W, c = g * a.W + k % a.W;
+    // Lanes across the group's channels, the rest of the workgroup along its chunks, eight loads of each kind in flight.
+    const int across = a.W < kBlock ? static_cast<int>(a.W) : kBlock, slots = kBlock / across, slot = threadIdx.x / across;
+    for (int64_t in_group = threadIdx.x % across; in_group < a.W && slot < slots; in_group += across) {
+        const int64_t c = g * a.W + in_group;
         const double w = weight_of<T>(a.weight, c);
-        sum_h += w * in[part * a.C + c], sum += w * in[(parts + part) * a.C + c];
+        const C *rows = in + n * m.p.chunks * a.C + c;
+        constexpr int kAhead = 8;
+        for (int64_t k = slot; k < m.p.chunks; k += kAhead * slots) {
+            C d[kAhead], dh[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int64_t part = k + j * slots;
+                d[j] = dh[j] = 0;
+                if (part < m.p.chunks) dh[j] = rows[part * a.C], d[j] = rows[(parts + part) * a.C];
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) sum += w * d[j], sum_h += w * dh[j];
+        }
     }
     sum = lanes_sum(sum, 64), sum_h = lanes_sum(sum_h, 64);
     __shared__ double waves[2][kBlock / 64];
@@ -328,6 +371,7 @@ __global__ void __launch_bounds__(kBlock) apply_back_kernel(MapsArgs m, const do
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
     if (!at.on) return;
+    Walk<T, V, 2> walk(at, m.p, a.src, a.grad);
     C w[V], b[V], mean[V], rstd[V], d_mean[V], dh_mean[V];
     load_channels<T, V>(a.weight, at.c, C(1), w);
     load_channels<T, V>(a.bias, at.c, C(0), b);
@@ -338,11 +382,11 @@ __global__ void __launch_bounds__(kBlock) apply_back_kernel(MapsArgs m, const do
         d_mean[i] = static_cast<C>(p[0]), dh_mean[i] = static_cast<C>(p[1]);
     }
     T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
-    for_positions<T, V>(at, m.p, a.src, a.grad, [&](int64_t s, const Vec<T, V> &x, const Vec<T, V> &dy) {
+    walk.run([&](int64_t s, const Vec<T, V> &x, const Vec<T, V> &dy) {
         C hat[V], z[V];
         hat_and_slope<T, V>(m.activation, x, mean, rstd, w, b, hat, z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = rstd[i] * (w[i] * (dy.get(i) * z[i]) - d_mean[i] - hat[i] * dh_mean[i]);
+        for (int i = 0; i < V; ++i) z[i] = rstd[i] * fma_(-hat[i], dh_mean[i], w[i] * (dy.get(i) * z[i]) - d_mean[i]);
         Vec<T, V> dx;
         dx.round(z);
         dx.template store<PAST>(to + s * a.out.ss);
@@ -382,9 +426,9 @@ MapsPlan maps_plan(const NormArgs &a, int32_t dtype) {
     p.lanes = static_cast<int32_t>(across < kBlock ? across : kBlock);
     p.slots = kBlock / p.lanes;
     p.blocks = (across + p.lanes - 1) / p.lanes;
-    // Eight workgroups for every compute unit, but no chunk shorter than what a workgroup requests at once.
+    // Two workgroups for every compute unit (all of them resident), but no chunk shorter than what a workgroup requests at once.
     const int64_t shortest = kAtOnce * p.slots, most = (a.S + shortest - 1) / shortest;
-    int64_t chunks = (2048 + a.N * p.blocks - 1) / (a.N * p.blocks);
+    int64_t chunks = (512 + a.N * p.blocks - 1) / (a.N * p.blocks);
     chunks = chunks < 1 ? 1 : (chunks > most ? most : chunks);
     p.chunk = (a.S + chunks - 1) / chunks;
     p.chunks = (a.S + p.chunk - 1) / p.chunk;
@@ -409,7 +453,7 @@ int64_t norm_maps_room(const NormArgs &a, int32_t dtype, bool backward) {
 }
 
 bool queue_norm_maps(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward) {
-    if (a.src.sc != 1 || a.out.sc != 1 || (backward && a.grad.sc != 1) || !maps_fit(a, dtype)) return false;
+    if (!channels_adjacent(a, backward) || !maps_fit(a, dtype)) return false;
     MapsArgs m{a, maps_plan(a, dtype), activation, room};
     const bool past = a.N * a.S * a.C * dtype_size(dtype) * (backward ? 3 : 2) > kCacheResidentBytes;
     with_float_type(dtype, [&](auto tag) {

@@ -27,8 +27,8 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
     using C = typename Comp<T>::C;
     const NormArgs &a = s.a;
     const RowsPlan &p = s.p;
-    // Rows a lane works on at a time: about four vectors of each operand in flight.
-    constexpr int U = BACK ? (M == 1 ? 2 : 1) : (M <= 2 ? 4 / M : 1);
+    // Rows a lane works on at a time.
+    constexpr int U = !BACK && M == 1 ? 2 : 1;
     constexpr bool kKeep = M * V <= 16;  // the weights in registers
     const int tid = threadIdx.x, wave = tid >> 6, lane = WIDE ? tid : tid & 63;
     const int64_t block = blockIdx.x % p.blocks, walker = blockIdx.x / p.blocks;
@@ -70,6 +70,10 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
             for (int k = 0; k < kWaves; ++k) x += wide_sums[0][k], y += wide_sums[1][k];
         }
     };
+    // Many vectors are worked on one after the other: the scheduler would hold all their intermediate values at once.
+    auto one_by_one = [] {
+        if constexpr (M > 2) __builtin_amdgcn_sched_barrier(0);
+    };
     const double count = static_cast<double>(a.S) * static_cast<double>(a.W);
     C sum_d[BACK ? M : 1][V], sum_dh[BACK ? M : 1][V];
     if constexpr (BACK) {
@@ -79,25 +83,46 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
             for (int i = 0; i < V; ++i) sum_d[m][i] = sum_dh[m][i] = 0;
         }
     }
-    const int64_t stride = p.walkers * (WIDE ? 1 : kWaves) * U * p.rows;
-    for (int64_t n0 = (walker * (WIDE ? 1 : kWaves) + (WIDE ? 0 : wave)) * U * p.rows; n0 < a.N; n0 += stride) {
+    // The next rows are under way while these are worked on.
+    struct Rows {
         Vec<T, V> x[U][M], dy[BACK ? U : 1][M];
-        int64_t n[U];
+        C mean[U], rstd[U];  // backwards
         bool on[U];
+    };
+    auto fetch = [&](int64_t n0, Rows &rows) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            n[u] = n0 + u * p.rows + row;
-            on[u] = n[u] < a.N;
+            const int64_t n = n0 + u * p.rows + row;
+            rows.on[u] = n < a.N;
+            if constexpr (BACK) {
+                rows.mean[u] = rows.rstd[u] = 0;
+                if (rows.on[u] && slot_on) {
+                    rows.mean[u] = reinterpret_cast<const C *>(a.mean.p)[a.mean.at(n, g)];
+                    rows.rstd[u] = reinterpret_cast<const C *>(a.rstd.p)[a.rstd.at(n, g)];
+                }
+            }
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                x[u][m].only(false);
-                if constexpr (BACK) dy[u][m].only(false);
-                if (on[u] && at.on[m]) {
-                    x[u][m].template load<PAST>(reinterpret_cast<const T *>(a.src.p) + n[u] * a.src.sn + at.src[m]);
-                    if constexpr (BACK) dy[u][m].template load<PAST>(reinterpret_cast<const T *>(a.grad.p) + n[u] * a.grad.sn + at.grad[m]);
+                rows.x[u][m].only(false);
+                if constexpr (BACK) rows.dy[u][m].only(false);
+                if (rows.on[u] && at.on[m]) {
+                    rows.x[u][m].template load<PAST>(reinterpret_cast<const T *>(a.src.p) + n * a.src.sn + at.src[m]);
+                    if constexpr (BACK) rows.dy[u][m].template load<PAST>(reinterpret_cast<const T *>(a.grad.p) + n * a.grad.sn + at.grad[m]);
                 }
             }
         }
+    };
+    const int64_t stride = p.walkers * (WIDE ? 1 : kWaves) * U * p.rows;
+    int64_t n0 = (walker * (WIDE ? 1 : kWaves) + (WIDE ? 0 : wave)) * U * p.rows;
+    Rows next;
+    fetch(n0, next);
+    for (; n0 < a.N; n0 += stride) {
+        Rows now = next;
+        auto &x = now.x;
+        fetch(n0 + stride, next);
+        int64_t n[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) n[u] = n0 + u * p.rows + row;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             auto weights = [&](int m, C(&w)[V], C(&b)[V]) {
@@ -121,6 +146,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                         sum += v;
                         if constexpr (!std::is_same_v<T, double>) squares = __builtin_fma(v, v, squares);
                     }
+                    one_by_one();
                 }
                 group_sums(sum, squares);
                 const double mean = sum / count;
@@ -142,9 +168,13 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     variance = variance < 0 ? 0 : variance;
                 }
                 const double rstd = 1.0 / sqrt(variance + a.eps);
-                if (on[u] && slot_on && first == 0) {
+                if (now.on[u] && slot_on && first == 0) {
                     if (a.mean.p != nullptr) reinterpret_cast<C *>(a.mean.p)[a.mean.at(n[u], g)] = static_cast<C>(mean);
                     if (a.rstd.p != nullptr) reinterpret_cast<C *>(a.rstd.p)[a.rstd.at(n[u], g)] = static_cast<C>(rstd);
+                }
+                if constexpr (M > 2) {
+#pragma unroll
+                    for (int m = 0; m < M; ++m) x[u][m].forget();
                 }
                 const Centre<C> centre(mean);
                 const C scale = static_cast<C>(rstd);
@@ -153,17 +183,15 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     C w[V], b[V], z[V];
                     weights(m, w, b);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) z[i] = centre.from(x[u][m].get(i)) * scale * w[i] + b[i];
+                    for (int i = 0; i < V; ++i) z[i] = fma_(centre.from(x[u][m].get(i)) * scale, w[i], b[i]);
                     activate_all<V>(s.activation, z);
                     Vec<T, V> y;
                     y.round(z);
-                    if (on[u] && at.on[m]) y.template store<PAST>(reinterpret_cast<T *>(a.out.p) + n[u] * a.out.sn + at.out[m]);
+                    if (now.on[u] && at.on[m]) y.template store<PAST>(reinterpret_cast<T *>(a.out.p) + n[u] * a.out.sn + at.out[m]);
+                    one_by_one();
                 }
             } else {
-                C mean = 0, rstd = 0;
-                if (on[u] && slot_on) {
-                    mean = reinterpret_cast<const C *>(a.mean.p)[a.mean.at(n[u], g)], rstd = reinterpret_cast<const C *>(a.rstd.p)[a.rstd.at(n[u], g)];
-                }
+                const C mean = now.mean[u], rstd = now.rstd[u];
                 C hat[M][V], wd[M][V];
                 double wd_sum = 0, wdh_sum = 0;
 #pragma unroll
@@ -173,19 +201,20 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         hat[m][i] = (x[u][m].get(i) - mean) * rstd;
-                        z[i] = hat[m][i] * w[i] + b[i];
+                        z[i] = fma_(hat[m][i], w[i], b[i]);
                     }
                     slope_all<V>(s.activation, z);
                     C part = 0, part_h = 0;
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         // A lane without elements has a zero gradient (and a finite hat).
-                        const C d = on[u] && at.on[m] ? dy[u][m].get(i) * z[i] : C(0);
-                        sum_d[m][i] += d, sum_dh[m][i] += d * hat[m][i];
+                        const C d = now.on[u] && at.on[m] ? now.dy[u][m].get(i) * z[i] : C(0);
+                        sum_d[m][i] += d, sum_dh[m][i] = fma_(d, hat[m][i], sum_dh[m][i]);
                         wd[m][i] = w[i] * d;
-                        part += wd[m][i], part_h += wd[m][i] * hat[m][i];
+                        part += wd[m][i], part_h = fma_(wd[m][i], hat[m][i], part_h);
                     }
                     wd_sum += part, wdh_sum += part_h;
+                    one_by_one();
                 }
                 group_sums(wd_sum, wdh_sum);
                 const C d_mean = static_cast<C>(wd_sum / count), dh_mean = static_cast<C>(wdh_sum / count);
@@ -193,10 +222,10 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                 for (int m = 0; m < M; ++m) {
                     C r[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) r[i] = rstd * (wd[m][i] - d_mean - hat[m][i] * dh_mean);
+                    for (int i = 0; i < V; ++i) r[i] = rstd * fma_(-hat[m][i], dh_mean, wd[m][i] - d_mean);
                     Vec<T, V> dx;
                     dx.round(r);
-                    if (on[u] && at.on[m]) dx.template store<PAST>(reinterpret_cast<T *>(a.out.p) + n[u] * a.out.sn + at.out[m]);
+                    if (now.on[u] && at.on[m]) dx.template store<PAST>(reinterpret_cast<T *>(a.out.p) + n[u] * a.out.sn + at.out[m]);
                 }
             }
         }
@@ -242,8 +271,9 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 
 // ---- the weights' gradients ---------------------------------------------------------------------------------------------
 //
-// A workgroup adds up 32 channels: eight threads a channel take every eighth part in order, then the eight are added.
-constexpr int kSumChannels = 32, kSumSlices = kBlock / kSumChannels;
+// A workgroup adds up 16 channels: sixteen threads a channel take every sixteenth part in order, eight of each sum in flight,
+// then the sixteen are added.
+constexpr int kSumChannels = 16, kSumSlices = kBlock / kSumChannels;
 
 template <class T>
 __global__ void __launch_bounds__(kBlock) weights_sum_kernel(NormArgs a, const typename Comp<T>::C *partial, int64_t parts) {
@@ -253,10 +283,17 @@ __global__ void __launch_bounds__(kBlock) weights_sum_kernel(NormArgs a, const t
     const int64_t c = static_cast<int64_t>(blockIdx.x) * kSumChannels + in;
     double total[2] = {0, 0};
     if (c < a.C) {
-        for (int which = 0; which < 2; ++which) {
-            const C *p = partial + which * parts * a.C + c;
-#pragma unroll 8
-            for (int64_t k = slice; k < parts; k += kSumSlices) total[which] += p[k * a.C];
+        constexpr int kAhead = 8;
+        for (int64_t k = slice; k < parts; k += kAhead * kSumSlices) {
+            C x[2][kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int64_t part = k + j * kSumSlices;
+                x[0][j] = x[1][j] = 0;
+                if (part < parts) x[0][j] = partial[part * a.C + c], x[1][j] = partial[(parts + part) * a.C + c];
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) total[0] += x[0][j], total[1] += x[1][j];
         }
     }
     slices[0][slice][in] = total[0], slices[1][slice][in] = total[1];
@@ -356,7 +393,7 @@ int64_t norm_rows_room(const NormArgs &a, int32_t dtype, bool backward) {
 }
 
 bool queue_norm_rows(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward) {
-    if (a.src.sc != 1 || a.out.sc != 1 || (backward && a.grad.sc != 1)) return false;
+    if (!channels_adjacent(a, backward)) return false;
     RowsArgs s{a, rows_plan(a, dtype, backward), activation, nullptr};
     if (s.p.m == 0 || a.N == 0) return false;
     const bool weights = backward && (a.d_weight.p != nullptr || a.d_bias.p != nullptr);

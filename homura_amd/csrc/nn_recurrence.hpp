@@ -50,9 +50,6 @@ struct RecurrenceArgs {
     }
 };
 
-__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
-__device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
-
 // sigmoid(z) and 1 - sigmoid(z), each to within a few units of its own last place: the smaller of the two comes from
 // exp(-|z|) itself, not from a subtraction.
 __device__ __forceinline__ void sigmoid_pair(float z, float &a, float &rest) {

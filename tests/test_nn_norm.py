@@ -115,6 +115,15 @@ def test_a_mean_far_from_zero_and_an_outlying_first_element(N, S, C, G):
         ref.assert_within(values(rstd), want_rstd, 16 * c.u * want_rstd, dtype, "rstd with an outlier")
 
 
+@pytest.mark.parametrize("N, S, C, G", [(40, 1, 24, 3), (2, 700, 24, 3)])
+def test_strided_weights(N, S, C, G):
+    c = Case(DT.BF16, N, S, C, G, "silu", 27)
+    vectors = c.vectors
+    c.vectors = lambda: tuple(on_gpu(np.repeat(v, 2), DT.BF16).slice(0, 0, None, 2) for v in (c.weight, c.bias))
+    c.check()
+    c.vectors = vectors
+
+
 def test_equal_elements_and_nan():
     x = np.full((3, 4, 16), 2.5)
     x[1, 2, 5] = np.nan
