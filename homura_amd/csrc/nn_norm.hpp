@@ -162,23 +162,38 @@ __device__ __forceinline__ A lanes_sum(A v, int lanes) {
     return v;
 }
 
-// A mean as it is subtracted: in f32 as the nearest value and what is left, so that x - mean keeps its digits where x is
-// near a mean that is far from zero.
+// 1 / sqrt(v) of a f64 from the hardware's estimate and two Newton steps (an f64 square root and division take some
+// thirty-five instructions, this a dozen); 0 and infinity, where the steps make NaN of them, keep the estimate.
+__device__ __forceinline__ double reciprocal_root(double v) {
+    const double seed = __builtin_amdgcn_rsq(v);
+    double y = seed;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const double e = __builtin_fma(-v * y, y, 1.0);
+        y = __builtin_fma(0.5 * y, e, y);
+    }
+    return y == y ? y : seed;
+}
+
+// (x - mean) * rstd. In f32 the mean is subtracted as the nearest value and what is left of it, so that the difference
+// keeps its digits where x is near a mean that is far from zero.
 template <class C>
 struct Centre;
 template <>
 struct Centre<float> {
-    float near, rest;
+    float near, scale, rest;
     Centre() = default;
-    __device__ __forceinline__ explicit Centre(double mean) : near(static_cast<float>(mean)), rest(static_cast<float>(mean - static_cast<double>(near))) {}
-    __device__ __forceinline__ float from(float x) const { return (x - near) - rest; }
+    __device__ __forceinline__ Centre(double mean, double rstd) : near(static_cast<float>(mean)), scale(static_cast<float>(rstd)) {
+        rest = static_cast<float>(static_cast<double>(near) - mean) * scale;
+    }
+    __device__ __forceinline__ float hat(float x) const { return fma_(x - near, scale, rest); }
 };
 template <>
 struct Centre<double> {
-    double mean;
+    double mean, scale;
     Centre() = default;
-    __device__ __forceinline__ explicit Centre(double m) : mean(m) {}
-    __device__ __forceinline__ double from(double x) const { return x - mean; }
+    __device__ __forceinline__ Centre(double m, double rstd) : mean(m), scale(rstd) {}
+    __device__ __forceinline__ double hat(double x) const { return (x - mean) * scale; }
 };
 
 // The weights or biases of V channels, which lie next to each other; `otherwise` without a tensor.

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
     Walk<T, V, 1> walk(at, m.p, a.src, a.src);
-    C w[V], b[V], rstd[V];
+    C w[V], b[V];
     load_channels<T, V>(a.weight, at.on ? at.c : 0, C(1), w);
     load_channels<T, V>(a.bias, at.on ? at.c : 0, C(0), b);
     // The block's groups' means and reciprocal deviations.
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
         const int64_t k = k0 + threadIdx.x / lanes;
         const Moments<T> all = gather<T>(m, at.n, k < groups ? g0 + k : g0, static_cast<int64_t>(m.p.lanes) * V, threadIdx.x % lanes, lanes, k < groups);
         if (k < groups && threadIdx.x % lanes == 0) {
-            const double mean = all.mean(less_of<T>(a, at.n, g0 + k)), rstd = 1.0 / sqrt(all.variance() + a.eps);
+            const double mean = all.mean(less_of<T>(a, at.n, g0 + k)), rstd = reciprocal_root(all.variance() + a.eps);
             statistics[k] = mean, statistics[room + k] = rstd;
             // One workgroup of the map writes a group's statistics: the first chunk's, in the block where the group begins.
             if (at.chunk == 0 && (g0 + k) * a.W >= at.c0) {
@@ -247,13 +247,13 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int64_t k = (at.c + i) / a.W - g0;
-        centre[i] = Centre<C>(statistics[k]), rstd[i] = static_cast<C>(statistics[room + k]);
+        centre[i] = Centre<C>(statistics[k], statistics[room + k]);
     }
     T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
     walk.run([&](int64_t s, const Vec<T, V> &x) {
         C z[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = fma_(centre[i].from(x.get(i)) * rstd[i], w[i], b[i]);
+        for (int i = 0; i < V; ++i) z[i] = fma_(centre[i].hat(x.get(i)), w[i], b[i]);
         activate_all<V>(m.activation, z);
         Vec<T, V> y;
         y.round(z);

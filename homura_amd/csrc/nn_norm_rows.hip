@@ -55,9 +55,10 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
             load_channels<T, V>(a.bias, at.channel[m], C(0), keep_b[m]);
         }
     }
-    __shared__ double wide_sums[2][kWaves];
-    // The sums of both over a group's lanes.
-    auto group_sums = [&](double &x, double &y) {
+    // The sums of both over a group's lanes: moments in f64, the gradient's two sums in the computation type.
+    using A = std::conditional_t<BACK, C, double>;
+    __shared__ A wide_sums[2][kWaves];
+    auto group_sums = [&](A &x, A &y) {
         if constexpr (!WIDE) {
             x = lanes_sum(x, p.lanes), y = lanes_sum(y, p.lanes);
         } else {
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
     auto one_by_one = [] {
         if constexpr (M > 2) __builtin_amdgcn_sched_barrier(0);
     };
-    const double count = static_cast<double>(a.S) * static_cast<double>(a.W);
+    const double share = 1.0 / (static_cast<double>(a.S) * static_cast<double>(a.W));
     C sum_d[BACK ? M : 1][V], sum_dh[BACK ? M : 1][V];
     if constexpr (BACK) {
 #pragma unroll
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     one_by_one();
                 }
                 group_sums(sum, squares);
-                const double mean = sum / count;
+                const double mean = sum * share;
                 double variance;
                 if constexpr (std::is_same_v<T, double>) {
                     double centred = 0, none = 0;
@@ -162,12 +163,12 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                         }
                     }
                     group_sums(centred, none);
-                    variance = centred / count;
+                    variance = centred * share;
                 } else {
-                    variance = __builtin_fma(-mean, mean, squares / count);
+                    variance = __builtin_fma(-mean, mean, squares * share);
                     variance = variance < 0 ? 0 : variance;
                 }
-                const double rstd = 1.0 / sqrt(variance + a.eps);
+                const double rstd = reciprocal_root(variance + a.eps);
                 if (now.on[u] && slot_on && first == 0) {
                     if (a.mean.p != nullptr) reinterpret_cast<C *>(a.mean.p)[a.mean.at(n[u], g)] = static_cast<C>(mean);
                     if (a.rstd.p != nullptr) reinterpret_cast<C *>(a.rstd.p)[a.rstd.at(n[u], g)] = static_cast<C>(rstd);
@@ -176,14 +177,13 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 #pragma unroll
                     for (int m = 0; m < M; ++m) x[u][m].forget();
                 }
-                const Centre<C> centre(mean);
-                const C scale = static_cast<C>(rstd);
+                const Centre<C> centre(mean, rstd);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     C w[V], b[V], z[V];
                     weights(m, w, b);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) z[i] = fma_(centre.from(x[u][m].get(i)) * scale, w[i], b[i]);
+                    for (int i = 0; i < V; ++i) z[i] = fma_(centre.hat(x[u][m].get(i)), w[i], b[i]);
                     activate_all<V>(s.activation, z);
                     Vec<T, V> y;
                     y.round(z);
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
             } else {
                 const C mean = now.mean[u], rstd = now.rstd[u];
                 C hat[M][V], wd[M][V];
-                double wd_sum = 0, wdh_sum = 0;
+                C wd_sum = 0, wdh_sum = 0;
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     C w[V], b[V], z[V];
@@ -207,8 +207,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     C part = 0, part_h = 0;
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        // A lane without elements has a zero gradient (and a finite hat).
-                        const C d = now.on[u] && at.on[m] ? now.dy[u][m].get(i) * z[i] : C(0);
+                        const C d = now.dy[u][m].get(i) * z[i];  // a lane without elements has zero gradients
                         sum_d[m][i] += d, sum_dh[m][i] = fma_(d, hat[m][i], sum_dh[m][i]);
                         wd[m][i] = w[i] * d;
                         part += wd[m][i], part_h = fma_(wd[m][i], hat[m][i], part_h);
@@ -217,7 +216,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     one_by_one();
                 }
                 group_sums(wd_sum, wdh_sum);
-                const C d_mean = static_cast<C>(wd_sum / count), dh_mean = static_cast<C>(wdh_sum / count);
+                const C d_mean = wd_sum * static_cast<C>(share), dh_mean = wdh_sum * static_cast<C>(share);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     C r[V];
