@@ -243,15 +243,16 @@ RowsPlan rows_plan(const NormArgs &a, int32_t dtype, bool backward);
 // ---- maps: groups spread over workgroups --------------------------------------------------------------------------------
 //
 // Larger groups take two passes over the maps, the second one out of the memory-side cache where they fit it. A
-// workgroup holds a run of positions (a chunk) of up to 256 vectors of channels: lane (r, l) walks every `slots`-th
-// position of its V channels. The first pass leaves each chunk's sums (per group forwards, per channel backwards), the
-// second one adds up what concerns it, in order, and writes.
+// workgroup takes every `chunks`-th run of positions of up to 256 vectors of channels, so that all of them together move
+// through memory in its order; lane (r, l) takes every `slots`-th position of a run and V channels of it. The first pass
+// leaves the workgroup's sums (per group forwards, per channel backwards), the second one adds up what concerns it, in
+// order, and writes.
 struct MapsPlan {
     int32_t v;
     int32_t lanes, slots;  // across channels and positions
     int64_t blocks;        // of channels
-    int64_t chunks;        // of positions of one map
-    int64_t chunk;         // positions of one
+    int64_t chunks;        // workgroups that share a block of channels of one map
+    int64_t run;           // positions that a workgroup takes at a time
 };
 MapsPlan maps_plan(const NormArgs &a, int32_t dtype);
 
@@ -261,8 +262,42 @@ bool queue_norm_maps(hipStream_t stream, int32_t dtype, const NormArgs &a, int32
 int64_t norm_rows_room(const NormArgs &a, int32_t dtype, bool backward);
 int64_t norm_maps_room(const NormArgs &a, int32_t dtype, bool backward);
 
-// Adds up `parts` rows of partial sums of C channels ([2][parts][C]: the weights', then the biases') into the gradients.
-void queue_weights_sum(hipStream_t stream, int32_t dtype, const NormArgs &a, const void *partial, int64_t parts);
+// The weights' gradients from `parts` rows of partial sums ([2][parts][C]: the weights', then the biases'). A workgroup of
+// kBlock lanes adds up 16 channels: sixteen threads a channel take every sixteenth part in order, eight of each sum in flight,
+// then the sixteen are added.
+constexpr int kSumChannels = 16, kSumSlices = kBlock / kSumChannels;
+
+template <class T>
+__device__ __forceinline__ void sum_channels(const NormArgs &a, const typename Comp<T>::C *partial, int64_t parts, int64_t block) {
+    using C = typename Comp<T>::C;
+    __shared__ double slices[2][kSumSlices][kSumChannels];
+    const int in = threadIdx.x % kSumChannels, slice = threadIdx.x / kSumChannels;
+    const int64_t c = block * kSumChannels + in;
+    double total[2] = {0, 0};
+    if (c < a.C) {
+        constexpr int kAhead = 8;
+        for (int64_t k = slice; k < parts; k += kAhead * kSumSlices) {
+            C x[2][kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int64_t part = k + j * kSumSlices;
+                x[0][j] = x[1][j] = 0;
+                if (part < parts) x[0][j] = partial[part * a.C + c], x[1][j] = partial[(parts + part) * a.C + c];
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) total[0] += x[0][j], total[1] += x[1][j];
+        }
+    }
+    slices[0][slice][in] = total[0], slices[1][slice][in] = total[1];
+    __syncthreads();
+    if (slice < 2 && c < a.C) {
+        double sum = 0;
+#pragma unroll
+        for (int k = 0; k < kSumSlices; ++k) sum += slices[slice][k][in];
+        const PerChannel &to = slice == 0 ? a.d_weight : a.d_bias;
+        if (to.p != nullptr) store_state<T>(to.p, c * to.sc, to.wide, static_cast<C>(sum));
+    }
+}
 
 }  // namespace nn
 }  // namespace hmr

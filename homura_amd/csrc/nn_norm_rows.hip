@@ -270,40 +270,9 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 
 // ---- the weights' gradients ---------------------------------------------------------------------------------------------
 //
-// A workgroup adds up 16 channels: sixteen threads a channel take every sixteenth part in order, eight of each sum in flight,
-// then the sixteen are added.
-constexpr int kSumChannels = 16, kSumSlices = kBlock / kSumChannels;
-
 template <class T>
 __global__ void __launch_bounds__(kBlock) weights_sum_kernel(NormArgs a, const typename Comp<T>::C *partial, int64_t parts) {
-    using C = typename Comp<T>::C;
-    __shared__ double slices[2][kSumSlices][kSumChannels];
-    const int in = threadIdx.x % kSumChannels, slice = threadIdx.x / kSumChannels;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * kSumChannels + in;
-    double total[2] = {0, 0};
-    if (c < a.C) {
-        constexpr int kAhead = 8;
-        for (int64_t k = slice; k < parts; k += kAhead * kSumSlices) {
-            C x[2][kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int64_t part = k + j * kSumSlices;
-                x[0][j] = x[1][j] = 0;
-                if (part < parts) x[0][j] = partial[part * a.C + c], x[1][j] = partial[(parts + part) * a.C + c];
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) total[0] += x[0][j], total[1] += x[1][j];
-        }
-    }
-    slices[0][slice][in] = total[0], slices[1][slice][in] = total[1];
-    __syncthreads();
-    if (slice < 2 && c < a.C) {
-        double sum = 0;
-#pragma unroll
-        for (int k = 0; k < kSumSlices; ++k) sum += slices[slice][k][in];
-        const PerChannel &to = slice == 0 ? a.d_weight : a.d_bias;
-        if (to.p != nullptr) store_state<T>(to.p, c * to.sc, to.wide, static_cast<C>(sum));
-    }
+    sum_channels<T>(a, partial, parts, blockIdx.x);
 }
 
 int power_of_two(int64_t at_least) {
@@ -403,17 +372,14 @@ bool queue_norm_rows(hipStream_t stream, int32_t dtype, const NormArgs &a, int32
         if (backward) launch_width<T, true>(stream, s, past);
         else launch_width<T, false>(stream, s, past);
     });
-    if (weights) queue_weights_sum(stream, dtype, a, room, s.p.walkers);
+    if (weights) {
+        with_float_type(dtype, [&](auto tag) {
+            using T = typename decltype(tag)::type;
+            weights_sum_kernel<T><<<static_cast<uint32_t>((a.C + kSumChannels - 1) / kSumChannels), kBlock, 0, stream>>>(
+                a, static_cast<const typename Comp<T>::C *>(room), s.p.walkers);
+        });
+    }
     return true;
-}
-
-void queue_weights_sum(hipStream_t stream, int32_t dtype, const NormArgs &a, const void *partial, int64_t parts) {
-    with_float_type(dtype, [&](auto tag) {
-        using T = typename decltype(tag)::type;
-        using C = typename Comp<T>::C;
-        weights_sum_kernel<T><<<static_cast<uint32_t>((a.C + kSumChannels - 1) / kSumChannels), kBlock, 0, stream>>>(
-            a, static_cast<const C *>(partial), parts);
-    });
 }
 
 }  // namespace nn
