@@ -152,19 +152,29 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     }
     slots_n[threadIdx.x] = n;
     __syncthreads();
-    // The slots of a channel, in order, by the first slot's lanes.
-    if (at.on && at.slot == 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            Moments<T> all{slots_n[threadIdx.x], slots_sum[threadIdx.x][i], slots_squares[threadIdx.x][i]};
-            for (int k = 1; k < m.p.slots; ++k) {
-                const int l = threadIdx.x + k * m.p.lanes;
-                all.add(Moments<T>{slots_n[l], slots_sum[l][i], slots_squares[l][i]});
-            }
-            slots_sum[threadIdx.x][i] = all.a, slots_squares[threadIdx.x][i] = all.b;
+    // The slots of a channel joined by `share` threads, then those; the result goes to the first slot's place.
+    __shared__ Moments<T> parts[kBlock];
+    const int channels = static_cast<int>(at.c1 - at.c0), share = channels < kBlock ? kBlock / channels : 1;
+    for (int k = threadIdx.x; k < channels * share; k += kBlock) {
+        const int c = k % channels;
+        Moments<T> all{0, 0, 0};
+        for (int slot = k / channels; slot < m.p.slots; slot += share) {
+            const int l = c / V + slot * m.p.lanes;
+            all.add(Moments<T>{slots_n[l], slots_sum[l][c % V], slots_squares[l][c % V]});
         }
+        if (share == 1) slots_sum[c / V][c % V] = all.a, slots_squares[c / V][c % V] = all.b;
+        else parts[k] = all;
     }
     __syncthreads();
+    if (share > 1) {
+        if (threadIdx.x < static_cast<unsigned>(channels)) {
+            const int c = threadIdx.x;
+            Moments<T> all = parts[c];
+            for (int k = 1; k < share; ++k) all.add(parts[c + k * channels]);
+            slots_sum[c / V][c % V] = all.a, slots_squares[c / V][c % V] = all.b;
+        }
+        __syncthreads();
+    }
     // The positions of the workgroup's runs.
     const int64_t rounds = a.S / (m.p.run * m.p.chunks), left = a.S - rounds * m.p.run * m.p.chunks - at.s0;
     const double positions = static_cast<double>(rounds * m.p.run + (left < 0 ? 0 : (left < m.p.run ? left : m.p.run)));
@@ -177,79 +187,61 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     }
 }
 
-// The moments of group g of map n, by `lanes` neighbouring threads of which this is `lane`, a power of two up to 64; in
-// every one of them the same.
+// The groups' means and reciprocal deviations, [N * G][2] of f64 behind the moments, a wave a group: in the second pass's
+// workgroups the same sums took longer than this launch does ([16, 4096, 320] bf16: 21 us with them).
 template <class T>
-__device__ __forceinline__ Moments<T> gather(const MapsArgs &m, int64_t n, int64_t g, int64_t block_channels, int lane, int lanes, bool on) {
+__global__ void __launch_bounds__(kBlock) statistics_kernel(MapsArgs m, double *statistics) {
+    using C = typename Comp<T>::C;
     const NormArgs &a = m.a;
-    const int64_t first = g * a.W / block_channels, last = ((g + 1) * a.W - 1) / block_channels;
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + threadIdx.x / 64;
+    if (group >= a.N * a.G) return;
+    const int64_t n = group / a.G, g = group - n * a.G, block_channels = static_cast<int64_t>(m.p.lanes) * m.p.v;
+    const int lane = threadIdx.x % 64;
     const Moments<T> *in = static_cast<const Moments<T> *>(m.room) + n * m.p.chunks * m.p.blocks * a.G + g;
     Moments<T> all{0, 0, 0};
-    if (on) {
+    for (int64_t b = g * a.W / block_channels; b <= ((g + 1) * a.W - 1) / block_channels; ++b) {
         constexpr int kAhead = 4;  // loads in flight
-        for (int64_t b = first; b <= last; ++b) {
-            for (int64_t k = lane; k < m.p.chunks; k += kAhead * lanes) {
-                Moments<T> some[kAhead];
+        for (int64_t k = lane; k < m.p.chunks; k += kAhead * 64) {
+            Moments<T> some[kAhead];
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    if (k + j * lanes < m.p.chunks) some[j] = in[((k + j * lanes) * m.p.blocks + b) * a.G];
-                }
+            for (int j = 0; j < kAhead; ++j) {
+                if (k + j * 64 < m.p.chunks) some[j] = in[((k + j * 64) * m.p.blocks + b) * a.G];
+            }
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    if (k + j * lanes < m.p.chunks) all.add(some[j]);
-                }
+            for (int j = 0; j < kAhead; ++j) {
+                if (k + j * 64 < m.p.chunks) all.add(some[j]);
             }
         }
     }
-    for (int d = 1; d < lanes; d <<= 1) {
-        Moments<T> other{__shfl_xor(all.n, d, 64), __shfl_xor(all.a, d, 64), __shfl_xor(all.b, d, 64)};
+    for (int d = 1; d < 64; d <<= 1) {
+        const Moments<T> other{__shfl_xor(all.n, d, 64), __shfl_xor(all.a, d, 64), __shfl_xor(all.b, d, 64)};
         // Joined lower lane first on both sides, so that they agree.
-        if (lane & d) {
-            Moments<T> low = other;
-            low.add(all);
-            all = low;
-        } else {
-            all.add(other);
-        }
+        Moments<T> low = lane & d ? other : all;
+        low.add(lane & d ? all : other);
+        all = low;
     }
-    return all;
+    if (lane != 0) return;
+    const double mean = all.mean(less_of<T>(a, n, g)), rstd = reciprocal_root(all.variance() + a.eps);
+    statistics[2 * group] = mean, statistics[2 * group + 1] = rstd;
+    if (a.mean.p != nullptr) reinterpret_cast<C *>(a.mean.p)[a.mean.at(n, g)] = static_cast<C>(mean);
+    if (a.rstd.p != nullptr) reinterpret_cast<C *>(a.rstd.p)[a.rstd.at(n, g)] = static_cast<C>(rstd);
 }
 
 template <class T, int V, bool PAST>
-__global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m) {
+__global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m, const double *statistics) {
     using C = typename Comp<T>::C;
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
+    if (!at.on) return;
     Walk<T, V, 1> walk(at, a, m.p, a.src, a.src);
     C w[V], b[V];
-    load_channels<T, V>(a.weight, at.on ? at.c : 0, C(1), w);
-    load_channels<T, V>(a.bias, at.on ? at.c : 0, C(0), b);
-    // The block's groups' means and reciprocal deviations.
-    extern __shared__ double statistics[];  // [2][groups of the block]
-    const int64_t g0 = at.c0 / a.W, groups = (at.c1 - 1) / a.W - g0 + 1, room = (m.p.lanes * V - 1) / a.W + 2;
-    int lanes = 64;
-    while (lanes > 1 && kBlock / lanes < groups) lanes /= 2;
-    const int each = kBlock / lanes;
-    for (int64_t k0 = 0; k0 < groups; k0 += each) {
-        const int64_t k = k0 + threadIdx.x / lanes;
-        const Moments<T> all = gather<T>(m, at.n, k < groups ? g0 + k : g0, static_cast<int64_t>(m.p.lanes) * V, threadIdx.x % lanes, lanes, k < groups);
-        if (k < groups && threadIdx.x % lanes == 0) {
-            const double mean = all.mean(less_of<T>(a, at.n, g0 + k)), rstd = reciprocal_root(all.variance() + a.eps);
-            statistics[k] = mean, statistics[room + k] = rstd;
-            // One workgroup of the map writes a group's statistics: the first chunk's, in the block where the group begins.
-            if (at.chunk == 0 && (g0 + k) * a.W >= at.c0) {
-                if (a.mean.p != nullptr) reinterpret_cast<C *>(a.mean.p)[a.mean.at(at.n, g0 + k)] = static_cast<C>(mean);
-                if (a.rstd.p != nullptr) reinterpret_cast<C *>(a.rstd.p)[a.rstd.at(at.n, g0 + k)] = static_cast<C>(rstd);
-            }
-        }
-    }
-    __syncthreads();
-    if (!at.on) return;
+    load_channels<T, V>(a.weight, at.c, C(1), w);
+    load_channels<T, V>(a.bias, at.c, C(0), b);
     Centre<C> centre[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int64_t k = (at.c + i) / a.W - g0;
-        centre[i] = Centre<C>(statistics[k], statistics[room + k]);
+        const double *p = statistics + 2 * (at.n * a.G + (at.c + i) / a.W);
+        centre[i] = Centre<C>(p[0], p[1]);
     }
     T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
     walk.run([&](int64_t s, const Vec<T, V> &x) {
@@ -314,16 +306,26 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
 #pragma unroll
     for (int i = 0; i < V; ++i) slots[0][threadIdx.x][i] = sum_h[i], slots[1][threadIdx.x][i] = sum[i];
     __syncthreads();
-    if (at.on && at.slot == 0) {
-        C *out = static_cast<C *>(m.room);
-        const int64_t parts = a.N * m.p.chunks, part = at.n * m.p.chunks + at.chunk;
-        for (int which = 0; which < 2; ++which) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
+    C *out = static_cast<C *>(m.room);
+    const int64_t rows = a.N * m.p.chunks, part = at.n * m.p.chunks + at.chunk;
+    __shared__ double parts[kBlock];
+    const int channels = static_cast<int>(at.c1 - at.c0), share = channels < kBlock ? kBlock / channels : 1;
+    for (int which = 0; which < 2; ++which) {
+        for (int k = threadIdx.x; k < channels * share; k += kBlock) {
+            const int c = k % channels;
+            double total = 0;
+            for (int slot = k / channels; slot < m.p.slots; slot += share) total += slots[which][c / V + slot * m.p.lanes][c % V];
+            if (share == 1) out[(which * rows + part) * a.C + at.c0 + c] = static_cast<C>(total);
+            else parts[k] = total;
+        }
+        if (share > 1) {
+            __syncthreads();
+            if (threadIdx.x < static_cast<unsigned>(channels)) {
                 double total = 0;
-                for (int k = 0; k < m.p.slots; ++k) total += slots[which][threadIdx.x + k * m.p.lanes][i];
-                out[(which * parts + part) * a.C + at.c + i] = static_cast<C>(total);
+                for (int k = 0; k < share; ++k) total += parts[threadIdx.x + k * channels];
+                out[(which * rows + part) * a.C + at.c0 + threadIdx.x] = static_cast<C>(total);
             }
+            __syncthreads();
         }
     }
 }
@@ -402,15 +404,20 @@ int64_t rows_bytes(const NormArgs &a, const MapsPlan &p, int32_t dtype) {
     return up16(2 * a.N * p.chunks * a.C * dtype_size(wide_type(dtype)));
 }
 
+int64_t moments_bytes(const NormArgs &a, const MapsPlan &p) {
+    return up16(a.N * p.chunks * p.blocks * a.G * static_cast<int64_t>(3 * sizeof(double)));
+}
+
 template <class T, int V>
 void launch_maps(hipStream_t stream, const MapsArgs &m, bool backward, bool past) {
     const NormArgs &a = m.a;
     const uint32_t groups = static_cast<uint32_t>(a.N * m.p.chunks * m.p.blocks);
     if (!backward) {
         moments_kernel<T, V><<<groups, kBlock, 0, stream>>>(m);
-        const size_t lds = 2 * sizeof(double) * static_cast<size_t>((m.p.lanes * V - 1) / a.W + 2);
-        if (past) apply_kernel<T, V, true><<<groups, kBlock, lds, stream>>>(m);
-        else apply_kernel<T, V, false><<<groups, kBlock, lds, stream>>>(m);
+        double *statistics = reinterpret_cast<double *>(static_cast<char *>(m.room) + moments_bytes(a, m.p));
+        statistics_kernel<T><<<static_cast<uint32_t>((a.N * a.G + kBlock / 64 - 1) / (kBlock / 64)), kBlock, 0, stream>>>(m, statistics);
+        if (past) apply_kernel<T, V, true><<<groups, kBlock, 0, stream>>>(m, statistics);
+        else apply_kernel<T, V, false><<<groups, kBlock, 0, stream>>>(m, statistics);
         return;
     }
     double *means = reinterpret_cast<double *>(static_cast<char *>(m.room) + rows_bytes(a, m.p, sizeof(T) == 2 ? HMR_BF16 : (sizeof(T) == 4 ? HMR_F32 : HMR_F64)));
@@ -453,8 +460,7 @@ bool maps_fit(const NormArgs &a, int32_t dtype) {
 int64_t norm_maps_room(const NormArgs &a, int32_t dtype, bool backward) {
     if (!maps_fit(a, dtype)) return 0;
     const MapsPlan p = maps_plan(a, dtype);
-    if (!backward) return a.N * p.chunks * p.blocks * a.G * static_cast<int64_t>(3 * sizeof(double));
-    return rows_bytes(a, p, dtype) + a.N * a.G * static_cast<int64_t>(2 * sizeof(double));
+    return (backward ? rows_bytes(a, p, dtype) : moments_bytes(a, p)) + a.N * a.G * static_cast<int64_t>(2 * sizeof(double));
 }
 
 bool queue_norm_maps(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward) {

@@ -11,7 +11,8 @@ struct RowsArgs {
     NormArgs a;
     RowsPlan p;
     int32_t activation;
-    void *partial;  // backwards: [2][walkers][C] sums in the computation type
+    bool weights;   // backwards: whether the weights' gradients are wanted,
+    void *partial;  // and room for [2][walkers][C] sums in the computation type
 };
 
 // Where a lane's vectors lie, the same for every row it visits.
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
         }
     }
     if constexpr (BACK) {
-        if (s.partial == nullptr) return;
+        if (!s.weights) return;
         // The lanes of one channel (a lane of every wave; of several positions and rows where those are side by side) are
         // added in order by the thread that owns the channel in the workgroup's block.
         constexpr int kSpread = WIDE ? kBlock : 64;
@@ -240,6 +241,13 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
         const int64_t c0 = block * side * a.W;
         const int64_t channels = (c0 + side * a.W < a.C ? c0 + side * a.W : a.C) - c0;
         const int positions = static_cast<int>(a.S);
+        __shared__ double parts[kBlock];
+        // A lone walker's sums are the gradients.
+        auto put = [&](int which, int64_t c, double total) {
+            const PerChannel &to = which == 0 ? a.d_weight : a.d_bias;
+            if (p.walkers > 1) partial[(which * p.walkers + walker) * a.C + c] = static_cast<C>(total);
+            else if (to.p != nullptr) store_state<T>(to.p, c * to.sc, to.wide, static_cast<C>(total));
+        };
         for (int which = 0; which < 2; ++which) {
             __syncthreads();
 #pragma unroll
@@ -250,19 +258,33 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                 }
             }
             __syncthreads();
-            for (int64_t c = tid; c < channels; c += kBlock) {
-                const int group = static_cast<int>(c / a.W), in = static_cast<int>(c - group * a.W);
+            // `share` threads a channel where there are fewer channels than threads.
+            const int entries = (WIDE ? 1 : kWaves) * p.rows * positions;
+            const int share = channels < kBlock && entries != kWaves ? kBlock / static_cast<int>(channels) : 1;
+            for (int64_t k = tid; k < channels * share; k += kBlock) {
+                const int c = static_cast<int>(k % channels), group = static_cast<int>(c / a.W), in = static_cast<int>(c - group * a.W);
                 double total = 0;
-                for (int w = 0; w < (WIDE ? 1 : kWaves); ++w) {
-                    for (int r = 0; r < p.rows; ++r) {
-                        for (int position = 0; position < positions; ++position) {
-                            const int j = position * p.per_position + in / V;
-                            const int l = (r * side + group) * p.lanes + j % p.lanes, m = j / p.lanes;
-                            total += sums[((static_cast<int64_t>(w) * M + m) * kSpread + l) * V + in % V];
-                        }
-                    }
+                auto add = [&](int w, int r, int position) {
+                    const int j = position * p.per_position + in / V;
+                    const int l = (r * side + group) * p.lanes + j % p.lanes, m = j / p.lanes;
+                    total += sums[((w * M + m) * kSpread + l) * V + in % V];
+                };
+                if (entries == kWaves) {  // a position and a row a wave: the usual tokens
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) add(w, 0, 0);
+                } else {
+                    for (int e = static_cast<int>(k / channels); e < entries; e += share) add(e / positions / p.rows, e / positions % p.rows, e % positions);
                 }
-                partial[(which * p.walkers + walker) * a.C + c0 + c] = static_cast<C>(total);
+                if (share == 1) put(which, c0 + c, total);
+                else parts[k] = total;
+            }
+            if (share > 1) {
+                __syncthreads();
+                if (tid < channels) {
+                    double total = 0;
+                    for (int k = 0; k < share; ++k) total += parts[tid + k * channels];
+                    put(which, c0 + tid, total);
+                }
             }
         }
     }
@@ -327,14 +349,16 @@ RowsPlan rows_plan(const NormArgs &a, int32_t dtype, bool backward) {
     RowsPlan p{};
     const int full = 16 / dtype_size(dtype);
     p.v = a.W % full == 0 ? full : (full == 8 && a.W % 2 == 0 ? 2 : 1);
-    if (a.S == 0 || a.W == 0 || a.S > 4096 || a.W > 65536) return p;
+    // Of maps only small ones: a group's channels at one position are short runs of memory (and, backwards, a channel's sum
+    // meets every position of it at the end).
+    if (a.S == 0 || a.W == 0 || a.S > 64 || a.W > 65536) return p;
     p.per_position = static_cast<int32_t>(a.W / p.v);
     const int64_t vectors = a.S * p.per_position;
     const int most = backward ? 4 : 8;  // vectors of a lane
     if (vectors <= 64 * most) {
         p.lanes = vectors < 64 ? power_of_two(vectors) : 64;
         p.m = power_of_two((vectors + p.lanes - 1) / p.lanes);
-    } else if (vectors <= kBlock * 4) {
+    } else if (a.S == 1 && vectors <= kBlock * 4) {
         p.wide = true, p.lanes = kBlock;
         p.m = vectors <= kBlock * 2 ? 2 : 4;
     } else {
@@ -362,17 +386,16 @@ int64_t norm_rows_room(const NormArgs &a, int32_t dtype, bool backward) {
 
 bool queue_norm_rows(hipStream_t stream, int32_t dtype, const NormArgs &a, int32_t activation, void *room, bool backward) {
     if (!channels_adjacent(a, backward)) return false;
-    RowsArgs s{a, rows_plan(a, dtype, backward), activation, nullptr};
-    if (s.p.m == 0 || a.N == 0) return false;
     const bool weights = backward && (a.d_weight.p != nullptr || a.d_bias.p != nullptr);
-    if (weights) s.partial = room;
+    RowsArgs s{a, rows_plan(a, dtype, backward), activation, weights, room};
+    if (s.p.m == 0 || a.N == 0) return false;
     const bool past = a.N * a.S * a.C * dtype_size(dtype) * (backward ? 3 : 2) > kCacheResidentBytes;
     with_float_type(dtype, [&](auto tag) {
         using T = typename decltype(tag)::type;
         if (backward) launch_width<T, true>(stream, s, past);
         else launch_width<T, false>(stream, s, past);
     });
-    if (weights) {
+    if (weights && s.p.walkers > 1) {
         with_float_type(dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
             weights_sum_kernel<T><<<static_cast<uint32_t>((a.C + kSumChannels - 1) / kSumChannels), kBlock, 0, stream>>>(

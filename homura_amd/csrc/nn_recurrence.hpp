@@ -149,7 +149,7 @@ struct ScanArgs {
 };
 
 // The largest tile of any shape in use, and the workgroups of a launch.
-constexpr int64_t kMostSteps = 256, kMostChannels = 256, kMostTiles = (int64_t{1} << 31) - 1;
+constexpr int64_t kMostSteps = 512, kMostChannels = 256, kMostTiles = (int64_t{1} << 31) - 1;
 
 // What a scan's launch goes by besides sizes: whether every sequence's channels lie next to each other, and whether every
 // row of them begins a cache line.

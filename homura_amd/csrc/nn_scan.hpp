@@ -305,6 +305,9 @@ template <class T, bool BACK>
 using LongShape = ScanShape<T, kVector<T>, BACK ? 32 : 16, BACK ? 4 : 6>;
 template <class T>
 using LoneShape = ScanShape<T, 1, kSlots, 8>;
+// Of up to eight channels in all, whatever their places: longer tiles.
+template <class T>
+using FewShape = ScanShape<T, 1, 64, 8>;
 
 // Queues a scan of this shape.
 template <class Shape, class T, int FORM, bool BACK, int PASSING>
@@ -332,6 +335,7 @@ void with_scan_shapes(int64_t steps, F &&f) {
         f(LongShape<T, true>{});
     }
     f(LoneShape<T>{});
+    f(FewShape<T>{});
 }
 
 template <bool BACK>
@@ -340,7 +344,9 @@ void queue_scan(hipStream_t stream, int32_t dtype, int32_t form, const Recurrenc
         using T = typename decltype(tag)::type;
         with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {
             constexpr int FORM = decltype(f)::value;
-            if (!layout.adjacent || a.C < kVector<T>) {
+            if (a.C <= FewShape<T>::kChannels && (!layout.adjacent || a.C < kVector<T>)) {
+                launch_scan<FewShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
+            } else if (!layout.adjacent || a.C < kVector<T>) {
                 launch_scan<LoneShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
             } else if (a.T <= kShortest) {
                 launch_scan<ShortShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
