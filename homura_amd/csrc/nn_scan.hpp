@@ -99,10 +99,10 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     // Where a tile lies.
     struct Tile {
         int64_t b, k, block;
-        int64_t steps;  // of its sequence
-        int64_t c0;     // the block's first channel
-        bool lane_on;   // whether the lane has channels,
-        int at;         // and its first one's place in the block
+        int64_t steps;   // of its sequence
+        int64_t c0, c1;  // the block's channels
+        bool lane_on;    // whether the lane has channels,
+        int at;          // and its first one's place in the block
         // The lane's steps from `from` to `to` lie inside the sequence, those from `end` on past the batch's last; `first`
         // is the sequence's first step (if it is the lane's at all), which backwards starts from `initial`.
         int from, to, end, first;
@@ -114,12 +114,14 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
         const int64_t of_sequence = ticket - t.b * (s.p.blocks * s.p.tiles);
         t.k = divide(static_cast<uint32_t>(of_sequence), s.p.by_blocks), t.block = of_sequence - t.k * s.p.blocks;
         t.steps = a.steps(t.b);
-        // A vector never crosses the last channel: the last block begins early enough to have one, the last lane's moves
-        // back over its neighbour's channels, and both compute the same for those.
-        t.c0 = t.block * CL;
-        if (V > 1 && t.c0 > a.C - V) t.c0 = a.C - V;
-        t.lane_on = t.c0 + l * V < a.C;
-        const int64_t c = V > 1 && t.c0 + l * V > a.C - V ? a.C - V : t.c0 + l * V;
+        // A vector never crosses the last channel: the last block begins early enough to have one, and the block before it
+        // ends there, so that no channel is two workgroups' (a state may be read and written in one place). Inside a
+        // block the last lane's vector moves back over its neighbour's channels, and both compute the same for those.
+        const int64_t last = V > 1 && (s.p.blocks - 1) * CL > a.C - V ? a.C - V : (s.p.blocks - 1) * CL;  // block's first channel
+        t.c0 = t.block + 1 < s.p.blocks ? t.block * CL : last;
+        t.c1 = t.block + 1 < s.p.blocks ? (t.c0 + CL < last ? t.c0 + CL : last) : a.C;
+        t.lane_on = t.c0 + l * V < t.c1;
+        const int64_t c = V > 1 && t.c0 + l * V > t.c1 - V ? t.c1 - V : t.c0 + l * V;
         t.at = static_cast<int>(c - t.c0);
         const int64_t q0 = t.k * TT + r * S;
         t.end = clamped(a.T - q0);
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     Raw now;
     load(t, now);
     const int64_t cj = t.c0 + tid;  // the channel whose slots this thread folds
-    const bool folds = tid < CL && cj < a.C;
+    const bool folds = tid < CL && cj < t.c1;
     C carry = 0;  // of channel cj: the value that enters the tile, then the one that leaves it
     if (folds && t.k == 0 && a.entry.p != nullptr) carry = load_state<T>(a.entry.p, a.entry.at(t.b, cj), a.entry.wide);
     // The lane's steps as maps, and their fold. The maps are computed again when the steps are run.
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
             publish(entries + t.k * CL * W + tid * W, tile_f, tile_u);
             fold_entries(entries + first * CL * W, tid * W, CL * W, static_cast<uint32_t>(t.k - first), group_f, group_u);
             if (t.k + 1 == first + s.p.group) publish(groups + g * CL * W + tid * W, group_f * tile_f, carried(tile_f, group_u, tile_u));
-        } else if (tid >= CL && tid < 2 * CL && t.c0 + tid - CL < a.C) {
+        } else if (tid >= CL && tid < 2 * CL && t.c0 + tid - CL < t.c1) {
             // The groups before this one, from the first one's constant on.
             C any = 1, state = 0;
             fold_entries(groups, (tid - CL) * W, CL * W, static_cast<uint32_t>(g), any, state);

@@ -241,6 +241,44 @@ def test_gradients_against_differences(is_sigmoid):
             assert abs((loss(*plus) - loss(*minus)) / (2 * e) - (got[k] * v).sum()) < e * e * 1e4 + 1e-13 * np.abs(got[k] * v).sum() / e + 1e-7
 
 
+@pytest.mark.parametrize("T", [1, 3, 40, 700])
+@pytest.mark.parametrize("C", [40, 259, 515, 1027])
+def test_a_state_read_and_written_in_one_place(T, C):
+    """last is initial, d_initial is grad_last: also where the number of channels leaves the last block of a scan a few,
+    less than a vector."""
+    from ctypes import byref, c_int64
+
+    from homura_amd import capi
+    B = 3
+    c = Case(DT.BF16, B, T, C, True, 91)
+    state = ref.rounded(ref.recurrence(c.gate, c.x, c.initial, None, True, c.u)[0], DT.BF16)
+    grad = ref.rounded(normal(6, B * T * C).reshape(B, T, C), DT.BF16)
+    grad_last = ref.rounded(normal(7, B * C).reshape(B, C), DT.F32)
+    want = ref.recurrence(c.gate, c.x, c.initial, None, True, c.u)
+    back, bounds = ref.recurrence_backward(grad, grad_last, c.gate, c.x, state, c.initial, None, True, c.u)
+    ctx = capi.Context(0)
+    try:
+        put = {k: ctx.upload(from_f64(v, DT.BF16)) for k, v in (("gate", c.gate), ("x", c.x), ("state", state), ("grad", grad))}
+        put.update({k: ctx.malloc(2 * B * T * C) for k in ("out", "d_gate", "d_x")})
+        put["at"], put["g"], put["from"] = (ctx.upload(v.astype(np.float32)) for v in (c.initial, grad_last, c.initial))
+        d = {k: byref(capi.make_desc(b.ptr, capi.BF16, (B, T, C), (T * C, C, 1))) for k, b in put.items()}
+        d.update({k: byref(capi.make_desc(put[k].ptr, capi.F32, (B, C), (C, 1))) for k in ("at", "g", "from")})
+        need = c_int64(0)
+        capi.check_nn(capi.nn.hmn_recurrence_workspace(d["x"], byref(need)))
+        room = ctx.malloc(need.value)
+        capi.check_nn(capi.nn.hmn_recurrence(ctx.handle, 1, d["out"], d["at"], d["gate"], d["x"], d["at"], None, room.ptr, need.value))
+        capi.check_nn(capi.nn.hmn_recurrence_backward(ctx.handle, 1, d["d_gate"], d["d_x"], d["g"], d["grad"], d["g"], d["gate"], d["x"],
+                                                      d["state"], d["from"], None, room.ptr, need.value))
+        ref.assert_within(to_f64(put["out"].download(np.uint16, B * T * C), DT.BF16).reshape(B, T, C), want[0], want[2], DT.BF16, "out")
+        ref.assert_within(put["at"].download(np.float32, B * C).reshape(B, C), want[1], want[3], DT.F32, "last")
+        ref.assert_within(put["g"].download(np.float32, B * C).reshape(B, C), back["d_initial"], bounds["d_initial"], DT.F32, "d_initial")
+        for k, name in (("d_gate", "d_gate"), ("d_x", "d_input")):
+            got = to_f64(put[k].download(np.uint16, B * T * C), DT.BF16).reshape(B, T, C)
+            ref.assert_within(got, back[name], bounds[name], DT.BF16, name)
+    finally:
+        ctx.close()
+
+
 def test_infinities_and_nan_stay_in_their_channel():
     B, T, C = 1, 300, 16
     c = Case(DT.F32, B, T, C, False, 71)
