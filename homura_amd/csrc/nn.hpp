@@ -62,6 +62,9 @@ inline hmr_status check_room(const char *who, const void *workspace, int64_t hav
     return HMR_OK;
 }
 
+// A launch has fewer than 2^32 threads; what would take more goes to kernels that loop.
+inline bool fits_launch(int64_t groups, int block) { return groups < (int64_t{1} << 32) / block; }
+
 // ---- device side --------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }

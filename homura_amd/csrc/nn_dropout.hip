@@ -162,7 +162,7 @@ bool queue_rows(hipStream_t stream, const DropoutArgs &a) {
         }
     }
     const int64_t groups = (s.vectors + kBlock - 1) / kBlock;
-    if (groups >= int64_t{1} << 31) return false;
+    if (!fits_launch(groups, kBlock)) return false;
     const uint32_t grid = static_cast<uint32_t>(groups);
     const bool past = a.n * static_cast<int64_t>(sizeof(T)) * operands > kCacheResidentBytes;
     if (residual) {

@@ -81,7 +81,8 @@ __device__ __forceinline__ C slope(C z) {
         return C(0.5) * erfc(-z * C(kRootHalf)) + z * exp(C(-0.5) * z * z) * C(0.5 * kRootTwoByPi);
     } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
         const C q = tanh_gate(z);
-        return fma_(z * q * (C(1) - q), fma_(C(6 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)), q);
+        // Far out, where q (1 - q) is zero, z^2 is kept finite.
+        return fma_(z * q * (C(1) - q), fma_(C(6 * kRootTwoByPi * kTanhInner), fmin(z * z, C(1e30)), C(2 * kRootTwoByPi)), q);
     } else {
         return C(1);
     }

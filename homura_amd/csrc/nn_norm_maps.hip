@@ -113,7 +113,8 @@ struct Walk {
 
 // ---- forwards ---------------------------------------------------------------------------------------------------------
 
-// [N][chunks][blocks][G] moments; a block writes those of the groups it has channels of.
+// [N][chunks][G + blocks] moments; block b writes those of the groups g that it has channels of, at b + g (of two blocks
+// one group at most is both's).
 template <class T, int V>
 __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     const NormArgs &a = m.a;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     // The positions of the workgroup's runs.
     const int64_t rounds = a.S / (m.p.run * m.p.chunks), left = a.S - rounds * m.p.run * m.p.chunks - at.s0;
     const double positions = static_cast<double>(rounds * m.p.run + (left < 0 ? 0 : (left < m.p.run ? left : m.p.run)));
-    Moments<T> *out = static_cast<Moments<T> *>(m.room) + ((at.n * m.p.chunks + at.chunk) * m.p.blocks + at.block) * a.G;
+    Moments<T> *out = static_cast<Moments<T> *>(m.room) + (at.n * m.p.chunks + at.chunk) * (a.G + m.p.blocks) + at.block;
     for (int64_t g = at.c0 / a.W + threadIdx.x; g * a.W < at.c1; g += kBlock) {
         const int64_t from = g * a.W > at.c0 ? g * a.W : at.c0, to = (g + 1) * a.W < at.c1 ? (g + 1) * a.W : at.c1;
         Moments<T> all{0, 0, 0};
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(kBlock) statistics_kernel(MapsArgs m, double *
     if (group >= a.N * a.G) return;
     const int64_t n = group / a.G, g = group - n * a.G, block_channels = static_cast<int64_t>(m.p.lanes) * m.p.v;
     const int lane = threadIdx.x % 64;
-    const Moments<T> *in = static_cast<const Moments<T> *>(m.room) + n * m.p.chunks * m.p.blocks * a.G + g;
+    const Moments<T> *in = static_cast<const Moments<T> *>(m.room) + n * m.p.chunks * (a.G + m.p.blocks) + g;
     Moments<T> all{0, 0, 0};
     for (int64_t b = g * a.W / block_channels; b <= ((g + 1) * a.W - 1) / block_channels; ++b) {
         constexpr int kAhead = 4;  // loads in flight
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kBlock) statistics_kernel(MapsArgs m, double *
             Moments<T> some[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
-                if (k + j * 64 < m.p.chunks) some[j] = in[((k + j * 64) * m.p.blocks + b) * a.G];
+                if (k + j * 64 < m.p.chunks) some[j] = in[(k + j * 64) * (a.G + m.p.blocks) + b];
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
@@ -405,7 +406,7 @@ int64_t rows_bytes(const NormArgs &a, const MapsPlan &p, int32_t dtype) {
 }
 
 int64_t moments_bytes(const NormArgs &a, const MapsPlan &p) {
-    return up16(a.N * p.chunks * p.blocks * a.G * static_cast<int64_t>(3 * sizeof(double)));
+    return up16(a.N * p.chunks * (a.G + p.blocks) * static_cast<int64_t>(3 * sizeof(double)));
 }
 
 template <class T, int V>
@@ -453,7 +454,7 @@ bool maps_fit(const NormArgs &a, int32_t dtype) {
     if (a.N == 0 || a.S == 0 || a.C == 0) return false;
     if (a.S < 8 && a.N * a.C > (int64_t{1} << 22)) return false;
     const MapsPlan p = maps_plan(a, dtype);
-    return a.N * p.chunks * p.blocks < (int64_t{1} << 31) && a.N * a.G + a.C < (int64_t{1} << 31);
+    return fits_launch(a.N * p.chunks * p.blocks, kBlock) && fits_launch(a.N * a.G + a.C, kBlock);
 }
 }  // namespace
 

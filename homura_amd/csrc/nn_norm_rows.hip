@@ -375,6 +375,7 @@ RowsPlan rows_plan(const NormArgs &a, int32_t dtype, bool backward) {
     int64_t walkers = (target + p.blocks - 1) / p.blocks;
     const int64_t useful = (a.N + rows_at_once - 1) / rows_at_once;
     p.walkers = walkers < useful ? walkers : (useful > 0 ? useful : 1);
+    if (!fits_launch(p.blocks * p.walkers, kBlock)) p.m = 0;
     return p;
 }
 

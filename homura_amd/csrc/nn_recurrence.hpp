@@ -148,8 +148,8 @@ struct ScanArgs {
     uint64_t *room;
 };
 
-// The largest tile of any shape in use, and the workgroups of a launch.
-constexpr int64_t kMostSteps = 512, kMostChannels = 256, kMostTiles = (int64_t{1} << 31) - 1;
+// The largest tile of any shape in use.
+constexpr int64_t kMostSteps = 512, kMostChannels = 256;
 
 // What a scan's launch goes by besides sizes: whether every sequence's channels lie next to each other, and whether every
 // row of them begins a cache line.

@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     const bool folds = tid < CL && cj < t.c1;
     C carry = 0;  // of channel cj: the value that enters the tile, then the one that leaves it
     if (folds && t.k == 0 && a.entry.p != nullptr) carry = load_state<T>(a.entry.p, a.entry.at(t.b, cj), a.entry.wide);
-    // The lane's steps as maps, and their fold. The maps are computed again when the steps are run.
+    // The lane's steps as maps, and their fold: what it adds is the state from zero exactly as steps one by one leave it
+    // (a zero times a factor that is not finite is NaN). The maps are computed again when the steps are run.
     auto map = [&](int i, int j, C &f, C &add) {
         const C z = now.gate[i].get(j);
         if constexpr (!BACK) {
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
         for (int j = 0; j < V; ++j) {
             C f, add;
             map(i, j, f, add);
-            fold_u[j] = i == 0 ? add : fma_(f, fold_u[j], add);
+            fold_u[j] = fma_(f, i == 0 ? C(0) : fold_u[j], add);
             fold_f[j] = i == 0 ? f : fold_f[j] * f;
         }
     }

@@ -27,7 +27,7 @@ int64_t most_of(const hmr_tensor_desc *gate, F measure) {
 
 bool scan_used(const hmr_tensor_desc *gate) {
     return gate->sizes[1] > kFewSteps && gate->sizes[0] > 0 && gate->sizes[2] > 0 &&
-           most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }) <= kMostTiles;
+           fits_launch(most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }), kScanBlock);
 }
 
 int64_t room_for(const hmr_tensor_desc *gate) {

@@ -45,8 +45,9 @@ const char *hmn_last_error(void);
  * be `initial` itself. With T = 1 the call is one step of decoding, with T = 0 it copies the state.
  *
  * A scan folds stretches of steps into (product of factors, state from zero), so a product of factors beyond the
- * computation type's range is infinite where step-by-step evaluation might not be: factors of magnitude at most one, as
- * gates are, never meet that.
+ * computation type's range is not finite where step-by-step evaluation might be, and one too small for it is zero. Factors
+ * of magnitude at most one, as gates are, never meet the first, and the second loses nothing of a state in any ordinary
+ * range.
  */
 #define HMN_GATE_FACTOR 0
 #define HMN_GATE_SIGMOID 1

@@ -216,6 +216,21 @@ def test_workspaces_are_asked_for_and_checked():
     refused(N.hmn_group_norm_workspace(byref(src), 5, 0, byref(need)), "5 groups")
 
 
+def test_workspaces_of_extreme_shapes():
+    """More workgroups than a launch has go without a scan; a group for every channel needs little more than the maps do."""
+    need = c_int64(-1)
+    for sizes in ((1 << 23, 5, 1), (1 << 22, 700, 1), (1 << 40, 5, 1)):
+        capi.check_nn(N.hmn_recurrence_workspace(byref(desc(capi.BF16, *sizes)), byref(need)))
+        assert need.value == 0
+    channels = 1 << 22
+    capi.check_nn(N.hmn_group_norm_workspace(byref(desc(capi.BF16, 1, 65, channels)), channels, 0, byref(need)))
+    assert 0 < need.value <= 48 * channels
+    for sizes, groups in (((1 << 24, 65, 8), 8), ((1 << 20, 65, 32), 32)):
+        for backward in (0, 1):
+            capi.check_nn(N.hmn_group_norm_workspace(byref(desc(capi.BF16, *sizes)), groups, backward, byref(need)))
+            assert need.value == 0
+
+
 def test_the_failure_text_belongs_to_the_thread_and_the_library():
     import threading
     refused(dropout(p=2.0), "probability")

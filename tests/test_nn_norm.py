@@ -124,6 +124,31 @@ def test_strided_weights(N, S, C, G):
     c.vectors = vectors
 
 
+@pytest.mark.parametrize("act", ACTIVATIONS)
+@pytest.mark.parametrize("N, S, C, G", [(40, 1, 24, 3), (2, 700, 24, 3)])
+def test_activations_far_out(N, S, C, G, act):
+    """Where the activation is z or zero and its slope one or zero, however large z is (its square is past F32's range)."""
+    c = Case(DT.F32, N, S, C, G, act, 25)
+    c.bias = np.where(np.arange(C) % 2 == 0, 1e25, -1e25)
+    w, b = c.vectors()
+    x = on_gpu(c.x, DT.F32)
+    out, mean, rstd = h.group_norm(x, G, w, b, c.eps, act)
+    z = np.broadcast_to(c.bias if act is None else np.maximum(c.bias, 0), c.x.shape)
+    assert (values(out) == np.float32(z)).all()  # |hat * weight| is less than half a step of 1e25
+    grads = h.grad_group_norm(on_gpu(c.grad, DT.F32), x, mean, rstd, G, w, b, act)
+    # The gradient of such an activation is that of none, with the zeroed channels' gradients gone.
+    grad = c.grad if act is None else np.where(c.bias > 0, c.grad, 0)
+    r, bounds = ref.group_norm_backward(grad, c.x, values(mean), values(rstd), G, c.weight, c.bias, None, c.u)
+    for got, name in zip(grads, ("d_x", "d_weight", "d_bias")):
+        ref.assert_within(values(got), r[name], bounds[name], DT.F32, name)
+
+
+def test_many_groups_of_one_channel_are_maps_too():
+    c = Case(DT.BF16, 1, 70, 4100, 4100, "silu", 26)
+    c.check()
+    Case(DT.F32, 2, 130, 2050, 1025, None, 27).check()
+
+
 def test_equal_elements_and_nan():
     x = np.full((3, 4, 16), 2.5)
     x[1, 2, 5] = np.nan

@@ -279,6 +279,15 @@ def test_a_state_read_and_written_in_one_place(T, C):
         ctx.close()
 
 
+def test_more_sequences_than_a_launch_has_workgroups():
+    """2^23 of them, a workgroup of 512 threads each, would be a launch of 2^32 threads."""
+    B, T = 1 << 23, 5
+    gate, x = (tensor(np.full(B * T, bits, dtype=np.uint16), DT.BF16, [B, T, 1], GPU) for bits in (0x3F00, 0x3F80))  # 0.5, 1
+    out, last = h.linear_recurrence(gate, x)
+    want = from_f64(np.array([1.0, 1.5, 1.75, 1.875, 1.9375]), DT.BF16)
+    assert (array(out).reshape(B, T) == want).all() and (values(last) == 1.9375).all()
+
+
 def test_infinities_and_nan_stay_in_their_channel():
     B, T, C = 1, 300, 16
     c = Case(DT.F32, B, T, C, False, 71)
@@ -292,6 +301,20 @@ def test_infinities_and_nan_stay_in_their_channel():
     rest = [k for k in range(C) if k not in (3, 5)]
     want, _, bound, _ = ref.recurrence(c.gate[..., rest], c.x[..., rest], None, None, False, c.u)
     ref.assert_within(out[..., rest], want, bound, DT.F32, "the other channels")
+
+
+@pytest.mark.parametrize("gate", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("T", [2, 16, 90, 700])
+def test_a_factor_that_is_not_finite_spoils_a_zero_state(T, gate):
+    """0 * inf and 0 * NaN are NaN, and NaN stays: whether the state is zero at the start or at a later step."""
+    for at in sorted({0, 1, T // 2, T - 1}):
+        c = Case(DT.F32, 2, T, 8, False, 72)
+        c.x[0, :at + 1, 2] = 0.0
+        c.gate[0, at, 2] = gate
+        out, last = (values(t) for t in h.linear_recurrence(on_gpu(c.gate, DT.F32), on_gpu(c.x, DT.F32)))
+        assert np.isnan(out[0, at:, 2]).all() and np.isnan(last[0, 2]) and (out[0, :at, 2] == 0).all()
+        out[0, :, 2] = 0
+        assert np.isfinite(out).all()
 
 
 def test_runs_repeat_bit_for_bit():
