@@ -1071,7 +1071,7 @@ void expect_nn(hmr_status s) {
     throw Error(message);
 }
 
-// The operand as it is, without merging dimensions: the entry points tell them apart.
+// The operand (of at most three dimensions) as it is, without merging any: the entry points tell them apart.
 hmr_tensor_desc whole_desc(const TensorData &t) {
     hmr_tensor_desc d;
     std::memset(&d, 0, sizeof d);
@@ -1158,9 +1158,11 @@ void group_norm_backward(const TensorData &d_src, const TensorData *d_weight, co
 }
 
 void dropout(const TensorData &out, const TensorData &src, const TensorData *residual, const DropoutMask &mask) {
-    const hmr_tensor_desc o = whole_desc(out), s = whole_desc(src);
-    const MaybeDesc r(residual);
-    exec(out, [&](hmr_context_t ctx) { expect_nn(hmn_dropout(ctx, &o, &s, r.get(), mask.p, mask.seed, mask.offset, nullptr)); });
+    std::vector<const TensorData *> operands = {&out, &src};
+    if (residual) operands.push_back(residual);
+    std::vector<hmr_tensor_desc> d;
+    if (!descs("dropout", operands, d)) return;
+    exec(out, [&](hmr_context_t ctx) { expect_nn(hmn_dropout(ctx, &d[0], &d[1], residual ? &d[2] : nullptr, mask.p, mask.seed, mask.offset, nullptr)); });
 }
 
 void upload(const TensorData &dst, const TensorData &src) {

@@ -125,5 +125,16 @@ def test_in_place_and_with_a_moved_base():
         ctx.close()
 
 
+def test_more_dimensions_than_a_description_holds():
+    shape = [1] * 20 + [2, 3] + [1] * 10 + [5, 1]
+    x = ref.rounded(normal(9, 30), DT.F32)
+    got, mask = h.dropout(on_gpu(x, DT.F32).reshape(shape), 0.5)
+    assert got.shape == shape and np.array_equal(values(got).ravel(), ref.dropout(x, None, *mask, DT.F32))
+    many = on_gpu(ref.rounded(normal(9, 1 << 13), DT.F32), DT.F32).reshape([2] * 13)
+    turned = many.permute(list(range(12, -1, -1)))
+    got, mask = h.dropout(turned, 0.5)
+    assert np.array_equal(values(got), ref.dropout(values(turned), None, *mask, DT.F32))
+
+
 def test_empty():
     assert h.dropout(on_gpu(np.zeros((3, 0)), DT.F32), 0.5)[0].shape == [3, 0]
