@@ -235,20 +235,22 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m, const double 
     const Place<V> at(a, m.p);
     if (!at.on) return;
     Walk<T, V, 1> walk(at, a, m.p, a.src, a.src);
-    C w[V], b[V];
+    // (x - near) * w + b, the weight with the reciprocal deviation and the bias with what the subtraction leaves of the mean.
+    C w[V], b[V], near[V];
     load_channels<T, V>(a.weight, at.c, C(1), w);
     load_channels<T, V>(a.bias, at.c, C(0), b);
-    Centre<C> centre[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const double *p = statistics + 2 * (at.n * a.G + (at.c + i) / a.W);
-        centre[i] = Centre<C>(p[0], p[1]);
+        near[i] = static_cast<C>(p[0]);
+        b[i] = static_cast<C>(__builtin_fma((static_cast<double>(near[i]) - p[0]) * p[1], static_cast<double>(w[i]), static_cast<double>(b[i])));
+        w[i] = static_cast<C>(p[1] * static_cast<double>(w[i]));
     }
     T *to = reinterpret_cast<T *>(a.out.p) + at.n * a.out.sn + at.c;
     walk.run([&](int64_t s, const Vec<T, V> &x) {
         C z[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = fma_(centre[i].hat(x.get(i)), w[i], b[i]);
+        for (int i = 0; i < V; ++i) z[i] = fma_(x.get(i) - near[i], w[i], b[i]);
         activate_all<V>(m.activation, z);
         Vec<T, V> y;
         y.round(z);
