@@ -86,7 +86,11 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     static_assert(TT <= kMostSteps && CL <= kMostChannels, "spans the host checks for");
     static_assert(2 * CL <= kScanBlock, "a thread per channel folds slots and tiles, another one groups");
     constexpr bool kLoadPast = PASSING == kPastCaches, kStorePast = PASSING != kThroughCaches;
+    // Many slots fold in two steps, runs of them by a thread each first.
+    constexpr int P = R > 32 ? 16 : R, RP = R / P;
+    static_assert(RP == 1 || P * CL <= kScanBlock, "a thread per channel and run of slots");
     __shared__ C slot_f[R][CL], slot_u[R][CL];
+    __shared__ C run_f[RP > 1 ? P : 1][CL], run_u[RP > 1 ? P : 1][CL];
     __shared__ C before_group[CHAIN ? CL : 1];
     __shared__ uint32_t drawn;
     const RecurrenceArgs &a = s.a;
@@ -210,17 +214,41 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
         for (int j = 0; j < V; ++j) slot_f[r][t.at + j] = fold_f[j], slot_u[r][t.at + j] = fold_u[j];
     }
     __syncthreads();
+    // The maps of this thread's channel: of the runs of slots, or of the slots themselves.
+    auto part_f = [&](int i) -> C & {
+        if constexpr (RP > 1) return run_f[i][tid];
+        else return slot_f[i][tid];
+    };
+    auto part_u = [&](int i) -> C & {
+        if constexpr (RP > 1) return run_u[i][tid];
+        else return slot_u[i][tid];
+    };
+    const int run_channel = tid % CL, run = tid / CL;
+    const bool has_run = RP > 1 && run < P && t.c0 + run_channel < t.c1;
+    if constexpr (RP > 1) {
+        if (has_run) {
+            C f = slot_f[run * RP][run_channel], u = slot_u[run * RP][run_channel];
+#pragma unroll
+            for (int i = 1; i < RP; ++i) {
+                const C nf = slot_f[run * RP + i][run_channel];
+                u = carried(nf, u, slot_u[run * RP + i][run_channel]);
+                f *= nf;
+            }
+            run_f[run][run_channel] = f, run_u[run][run_channel] = u;
+        }
+        __syncthreads();
+    }
     if constexpr (CHAIN) {
         const int64_t g = divide(static_cast<uint32_t>(t.k), s.p.by_group), first = g * s.p.group, chain = t.b * s.p.blocks + t.block;
         uint64_t *entries = s.room + 8 + chain * s.p.tiles * CL * W;
         uint64_t *groups = s.room + 8 + (a.B * s.p.blocks * s.p.tiles + chain * (s.p.tiles / s.p.group + 1)) * CL * W;
         C group_f = 1, group_u = 0;
         if (folds) {
-            C tile_f = slot_f[0][tid], tile_u = slot_u[0][tid];
+            C tile_f = part_f(0), tile_u = part_u(0);
 #pragma unroll 8
-            for (int i = 1; i < R; ++i) {
-                const C nf = slot_f[i][tid];
-                tile_u = carried(nf, tile_u, slot_u[i][tid]);
+            for (int i = 1; i < P; ++i) {
+                const C nf = part_f(i);
+                tile_u = carried(nf, tile_u, part_u(i));
                 tile_f *= nf;
             }
             // The first tile knows what enters it: its map is constant, and no other tile reads `entry`.
@@ -239,19 +267,31 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     }
     if (folds) {
         constexpr int kAhead = 8;
-        for (int i0 = 0; i0 < R; i0 += kAhead) {
+        for (int i0 = 0; i0 < P; i0 += kAhead) {
             C nf[kAhead], nu[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) nf[i] = slot_f[i0 + i][tid], nu[i] = slot_u[i0 + i][tid];
+            for (int i = 0; i < kAhead; ++i) nf[i] = part_f(i0 + i), nu[i] = part_u(i0 + i);
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                slot_u[i0 + i][tid] = carry;
+                part_u(i0 + i) = carry;
                 carry = carried(nf[i], carry, nu[i]);
             }
         }
         if (t.k + 1 == s.p.tiles && a.exit.p != nullptr) store_state<T>(a.exit.p, a.exit.at(t.b, cj), a.exit.wide, carry);
     }
     __syncthreads();
+    if constexpr (RP > 1) {
+        if (has_run) {
+            C into = run_u[run][run_channel];
+#pragma unroll
+            for (int i = 0; i < RP; ++i) {
+                const C nf = slot_f[run * RP + i][run_channel], nu = slot_u[run * RP + i][run_channel];
+                slot_u[run * RP + i][run_channel] = into;
+                into = carried(nf, into, nu);
+            }
+        }
+        __syncthreads();
+    }
     C e[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) e[j] = t.lane_on ? slot_u[r][t.at + j] : C(0);
@@ -306,6 +346,17 @@ template <class T>
 using ShortShape = ScanShape<T, kVector<T>, kSlots, 1>;
 template <class T, bool BACK>
 using LongShape = ScanShape<T, kVector<T>, BACK ? 32 : 16, BACK ? 4 : 6>;
+// Of few vectors of channels: the lanes that those would leave idle go along the sequence ([240, 8324, 8] f32 87 us, 387
+// with the long shape; [75, 906, 39] bf16 19 and 37). Of up to four blocks of channels (two backwards) too, where the long
+// shape would need several tiles ([240, 8324, 128] bf16 508 us and 638; backwards, 64 channels, 416 and 542, but 128
+// channels 799 and 662).
+template <class T>
+using NarrowShape = ScanShape<T, kVector<T>, 128, 4>;
+template <class T, bool BACK>
+bool narrow(const RecurrenceArgs &a) {
+    constexpr int64_t kOfBlock = NarrowShape<T>::kChannels;
+    return a.C <= kOfBlock || (a.T > LongShape<T, BACK>::kSteps && a.C <= (BACK ? 2 : 4) * kOfBlock);
+}
 template <class T>
 using LoneShape = ScanShape<T, 1, kSlots, 8>;
 // Of up to eight channels in all, whatever their places: longer tiles.
@@ -336,6 +387,7 @@ void with_scan_shapes(int64_t steps, F &&f) {
     } else {
         f(LongShape<T, false>{});
         f(LongShape<T, true>{});
+        f(NarrowShape<T>{});
     }
     f(LoneShape<T>{});
     f(FewShape<T>{});
@@ -353,6 +405,8 @@ void queue_scan(hipStream_t stream, int32_t dtype, int32_t form, const Recurrenc
                 launch_scan<LoneShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
             } else if (a.T <= kShortest) {
                 launch_scan<ShortShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
+            } else if (narrow<T, BACK>(a)) {
+                launch_scan<NarrowShape<T>, T, FORM, BACK, kThroughCaches>(stream, a, room);
             } else {
                 constexpr int64_t kOperands = BACK ? (FORM == HMN_GATE_SIGMOID ? 6 : 5) : 3;
                 const int64_t bytes = a.B * a.T * a.C * kOperands * static_cast<int64_t>(sizeof(T));

@@ -75,6 +75,15 @@ def test_forward_and_backward(B, T, C, dtype, is_sigmoid):
 
 
 @pytest.mark.parametrize("is_sigmoid", [False, True], ids=["factor", "sigmoid"])
+@pytest.mark.parametrize("dtype", FLOATS, ids=lambda d: d.name)
+@pytest.mark.parametrize("B, T, C", [(3, 60, 9), (2, 511, 8), (2, 513, 16), (4, 1100, 3), (2, 1100, 33), (2, 530, 39), (1, 1500, 64), (2, 600, 127)])
+def test_few_channels(B, T, C, dtype, is_sigmoid):
+    c = Case(dtype, B, T, C, is_sigmoid, seed=B * 1000 + T + C)
+    c.check_forward()
+    c.check_backward()
+
+
+@pytest.mark.parametrize("is_sigmoid", [False, True], ids=["factor", "sigmoid"])
 @pytest.mark.parametrize("dtype", [DT.BF16, DT.F32], ids=lambda d: d.name)
 @pytest.mark.parametrize("T, C", [(1, 24), (9, 24), (140, 72), (700, 19), (2100, 8)])
 def test_a_padded_batch(T, C, dtype, is_sigmoid):
