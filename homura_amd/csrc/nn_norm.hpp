@@ -61,13 +61,41 @@ __device__ __forceinline__ C tanh_gate(C z) {
     return logistic(z * fma_(C(2 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)));
 }
 
+// The normal distribution below z, and exp(-z^2 / 2). With a = |z| the tail beyond a is exp(-a^2 / 2) E(a), and E, which
+// falls slowly from 1/2 to 1 / (a sqrt(2 pi)), is t P(t) with t = 1 / (1 + 0.34 a): P is the polynomial of degree 8 of the
+// least relative error on a in 0..15, found by weighted least squares on 4000 Chebyshev points (half a unit of 2^-24; seven
+// as evaluated in f32, its 0.34 among the values that gave the least). The exponential's argument adds 1.5 z^2 units. With
+// the library's error function in its place [16384, 4096] bf16 took 118 us and its gradient for half as many rows 90, with
+// this 79 and 54.
+__device__ __forceinline__ void normal(float z, float &below, float &bell) {
+    constexpr float kP[9] = {0.135622576f, 0.13607347f, 0.115497872f, 0.114096098f, -0.041554004f, 0.197331294f, -0.26867196f, 0.137242302f, -0.0256376024f};
+    const float t = __builtin_amdgcn_rcpf(fma_(0.34f, fabsf(z), 1.0f));
+    bell = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    float p = kP[8];
+#pragma unroll
+    for (int k = 7; k >= 0; --k) p = fma_(p, t, kP[k]);
+    const float tail = bell * (t * p);
+    below = z < 0.0f ? tail : 1.0f - tail;
+}
+__device__ __forceinline__ void normal(double z, double &below, double &bell) {
+    below = 0.5 * erfc(-z * kRootHalf), bell = exp(-0.5 * z * z);
+}
+
 template <int ACT, class C>
 __device__ __forceinline__ C activate(C z) {
-    if constexpr (ACT == HMR_UNARY_RELU) return z < C(0) ? C(0) : z;
-    else if constexpr (ACT == HMR_UNARY_SILU) return z * logistic(z);
-    else if constexpr (ACT == HMR_UNARY_GELU) return C(0.5) * z * erfc(-z * C(kRootHalf));
-    else if constexpr (ACT == HMR_UNARY_GELU_TANH) return z * tanh_gate(z);
-    else return z;
+    if constexpr (ACT == HMR_UNARY_RELU) {
+        return z < C(0) ? C(0) : z;
+    } else if constexpr (ACT == HMR_UNARY_SILU) {
+        return z * logistic(z);
+    } else if constexpr (ACT == HMR_UNARY_GELU) {
+        C below, bell;
+        normal(z, below, bell);
+        return z * below;
+    } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
+        return z * tanh_gate(z);
+    } else {
+        return z;
+    }
 }
 
 template <int ACT, class C>
@@ -78,7 +106,9 @@ __device__ __forceinline__ C slope(C z) {
         const C q = logistic(z);
         return fma_(z * q, C(1) - q, q);
     } else if constexpr (ACT == HMR_UNARY_GELU) {
-        return C(0.5) * erfc(-z * C(kRootHalf)) + z * exp(C(-0.5) * z * z) * C(0.5 * kRootTwoByPi);
+        C below, bell;
+        normal(z, below, bell);
+        return fma_(z * bell, C(0.5 * kRootTwoByPi), below);
     } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
         const C q = tanh_gate(z);
         // Far out, where q (1 - q) is zero, z^2 is kept finite.
@@ -119,8 +149,8 @@ __device__ __forceinline__ void activate_all(int32_t activation, C (&z)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             z[i] = activate<decltype(act)::value>(z[i]);
-            // The error function's many intermediate values, of one element at a time.
-            if constexpr (decltype(act)::value == HMR_UNARY_GELU) __builtin_amdgcn_sched_barrier(0);
+            // The 64-bit error function's many intermediate values, of one element at a time.
+            if constexpr (decltype(act)::value == HMR_UNARY_GELU && sizeof(C) == 8) __builtin_amdgcn_sched_barrier(0);
         }
     });
 }
@@ -130,8 +160,8 @@ __device__ __forceinline__ void slope_all(int32_t activation, C (&z)[V]) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             z[i] = slope<decltype(act)::value>(z[i]);
-            // The error function's many intermediate values, of one element at a time.
-            if constexpr (decltype(act)::value == HMR_UNARY_GELU) __builtin_amdgcn_sched_barrier(0);
+            // The 64-bit error function's many intermediate values, of one element at a time.
+            if constexpr (decltype(act)::value == HMR_UNARY_GELU && sizeof(C) == 8) __builtin_amdgcn_sched_barrier(0);
         }
     });
 }

@@ -143,6 +143,23 @@ def test_activations_far_out(N, S, C, G, act):
         ref.assert_within(values(got), r[name], bounds[name], DT.F32, name)
 
 
+@pytest.mark.parametrize("dtype", [DT.F32, DT.F64], ids=lambda d: d.name)
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("S", [1, 80])
+def test_activations_over_their_range(S, act, dtype):
+    """A weight of zero makes z the bias itself: the activation and its slope, S times over, from -12 to 12."""
+    C, u = 2400, ref.COMPUTE[dtype]
+    z = ref.rounded(np.linspace(-12, 12, C), dtype)
+    w, b = on_gpu(np.zeros(C), dtype), on_gpu(z, dtype)
+    x, ones = on_gpu(normal(28, S * C).reshape(1, S, C), dtype), on_gpu(np.ones((1, S, C)), dtype)
+    out, mean, rstd = h.group_norm(x, 1, w, b, 1e-5, act)
+    y, slope, rel = ref.activate(z, act)
+    ref.assert_within(values(out), np.broadcast_to(y, (1, S, C)), np.broadcast_to((rel + 4) * u * np.abs(y), (1, S, C)), dtype, "out")
+    d_x, _, d_bias = h.grad_group_norm(ones, x, mean, rstd, 1, w, b, act)
+    assert (values(d_x) == 0).all()
+    ref.assert_within(values(d_bias), S * slope, S * (rel * u * (1 + np.abs(z)) + 64 * u * np.abs(slope)), dtype, "d_bias")
+
+
 def test_many_groups_of_one_channel_are_maps_too():
     c = Case(DT.BF16, 1, 70, 4100, 4100, "silu", 26)
     c.check()
