@@ -7,10 +7,10 @@ namespace {
 
 // ---- one thread per channel ----------------------------------------------------------------------------------
 //
-// Decoding and other sequences of a few steps: nothing to fold, one launch, the states in registers. Also steps so far apart
-// that a tile of the scan spans more than its 32-bit offsets (2 million elements of 16 bits: time-major batches with as
-// many channels in all, which keep the memory busy a thread each). `last` may be
-// `initial`: a channel's state is read and written by its own thread.
+// Decoding and other sequences of a few steps: nothing to fold, one launch, the states in registers ([64, 1, 4096] bf16 takes
+// 3.5 us, of which the memory would take one). Also steps so far apart that a tile of the scan spans more than its 32-bit
+// offsets (a million elements of 16 bits: time-major batches with as many channels in all, which keep the memory busy a
+// thread each). `last` may be `initial`: a channel's state is read and written by its own thread.
 
 template <class T, int FORM>
 __global__ void __launch_bounds__(kBlock) forward_kernel(RecurrenceArgs a) {

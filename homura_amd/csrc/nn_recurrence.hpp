@@ -159,8 +159,11 @@ struct ScanLayout {
 // Queue the scan of a direction (nn_scan_forward.hip, nn_scan_backward.hip). `room` holds room_for() bytes.
 void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, const ScanLayout &layout, void *room);
 void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, const ScanLayout &layout, void *room);
-// Sequences of up to this many steps go a thread per channel.
-constexpr int64_t kFewSteps = 4;
+// Sequences of so few steps go a thread per channel: there is nothing to gain in a scan of up to eight ([64, 6, 4096] bf16
+// 5 us, 10 by a scan), nor of up to 32 where there are enough channels to keep the chip busy, 2^16 of all sequences
+// ([512, 24, 4096] bf16 97 us and 168, backwards 145 and 315; [4096, 16, 40] 7 and 19; but [512, 16, 4096] f32 84 and 71, and
+// [512, 64, 4096] bf16 248 and 186).
+constexpr int64_t kFewSteps = 8, kFewWithMany = 32, kMany = int64_t{1} << 16;
 // Whether the sequences are long enough for a scan, and not too many for a launch with a workgroup for every tile.
 bool scan_used(const hmr_tensor_desc *gate);
 // Bytes of workspace of either direction, whatever the operands' strides.

@@ -359,7 +359,7 @@ bool narrow(const RecurrenceArgs &a) {
 }
 template <class T>
 using LoneShape = ScanShape<T, 1, kSlots, 8>;
-// Of up to eight channels in all, whatever their places: longer tiles.
+// Of up to eight channels in all, whatever their places: longer tiles ([64, 12964, 2] bf16 40 us, 175 with the lone shape).
 template <class T>
 using FewShape = ScanShape<T, 1, 64, 8>;
 

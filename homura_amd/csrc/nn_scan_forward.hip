@@ -26,8 +26,9 @@ int64_t most_of(const hmr_tensor_desc *gate, F measure) {
 }  // namespace
 
 bool scan_used(const hmr_tensor_desc *gate) {
-    return gate->sizes[1] > kFewSteps && gate->sizes[0] > 0 && gate->sizes[2] > 0 &&
-           fits_launch(most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }), kScanBlock);
+    if (gate->sizes[0] == 0 || gate->sizes[2] == 0 || gate->sizes[1] <= kFewSteps) return false;
+    if (gate->sizes[1] <= kFewWithMany && gate->sizes[0] >= (kMany + gate->sizes[2] - 1) / gate->sizes[2]) return false;
+    return fits_launch(most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }), kScanBlock);
 }
 
 int64_t room_for(const hmr_tensor_desc *gate) {

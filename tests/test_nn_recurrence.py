@@ -83,6 +83,14 @@ def test_few_channels(B, T, C, dtype, is_sigmoid):
     c.check_backward()
 
 
+@pytest.mark.parametrize("dtype", [DT.BF16, DT.F64], ids=lambda d: d.name)
+@pytest.mark.parametrize("B, T, C", [(256, 9, 256), (256, 32, 256), (256, 33, 256), (255, 32, 256), (3, 8, 40), (3, 9, 40), (3, 32, 40)])
+def test_few_steps(B, T, C, dtype):
+    c = Case(dtype, B, T, C, True, seed=B * 1000 + T + C)
+    c.check_forward()
+    c.check_backward()
+
+
 @pytest.mark.parametrize("is_sigmoid", [False, True], ids=["factor", "sigmoid"])
 @pytest.mark.parametrize("dtype", [DT.BF16, DT.F32], ids=lambda d: d.name)
 @pytest.mark.parametrize("T, C", [(1, 24), (9, 24), (140, 72), (700, 19), (2100, 8)])
@@ -288,13 +296,15 @@ def test_a_state_read_and_written_in_one_place(T, C):
         ctx.close()
 
 
-def test_more_sequences_than_a_launch_has_workgroups():
+@pytest.mark.parametrize("T", [5, 33])
+def test_more_sequences_than_a_launch_has_workgroups(T):
     """2^23 of them, a workgroup of 512 threads each, would be a launch of 2^32 threads."""
-    B, T = 1 << 23, 5
+    B = 1 << 23
     gate, x = (tensor(np.full(B * T, bits, dtype=np.uint16), DT.BF16, [B, T, 1], GPU) for bits in (0x3F00, 0x3F80))  # 0.5, 1
     out, last = h.linear_recurrence(gate, x)
-    want = from_f64(np.array([1.0, 1.5, 1.75, 1.875, 1.9375]), DT.BF16)
-    assert (array(out).reshape(B, T) == want).all() and (values(last) == 1.9375).all()
+    want = 2 - 2.0 ** -np.arange(T)
+    assert (array(out).reshape(B, T) == from_f64(want, DT.BF16)).all()
+    assert (array(last) == want[-1].astype(np.float32)).all()
 
 
 def test_infinities_and_nan_stay_in_their_channel():
