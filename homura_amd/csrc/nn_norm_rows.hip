@@ -48,13 +48,20 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
         at.src[m] = position * a.src.ss + at.channel[m], at.out[m] = position * a.out.ss + at.channel[m];
         at.grad[m] = BACK ? position * a.grad.ss + at.channel[m] : 0;
     }
+    // Backwards a vector without elements has weights and biases of zero: those of channel 0, which it would load, may be
+    // anything, and what it computes is added to its group's sums.
+    auto fetch_weights = [&](int m, C(&w)[V], C(&b)[V]) {
+        load_channels<T, V>(a.weight, at.channel[m], C(1), w);
+        load_channels<T, V>(a.bias, at.channel[m], C(0), b);
+        if constexpr (BACK) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = at.on[m] ? w[i] : C(0), b[i] = at.on[m] ? b[i] : C(0);
+        }
+    };
     C keep_w[kKeep ? M : 1][V], keep_b[kKeep ? M : 1][V];
     if constexpr (kKeep) {
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            load_channels<T, V>(a.weight, at.channel[m], C(1), keep_w[m]);
-            load_channels<T, V>(a.bias, at.channel[m], C(0), keep_b[m]);
-        }
+        for (int m = 0; m < M; ++m) fetch_weights(m, keep_w[m], keep_b[m]);
     }
     // The sums of both over a group's lanes: moments in f64, the gradient's two sums in the computation type.
     using A = std::conditional_t<BACK, C, double>;
@@ -132,8 +139,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) w[i] = keep_w[m][i], b[i] = keep_b[m][i];
                 } else {
-                    load_channels<T, V>(a.weight, at.channel[m], C(1), w);
-                    load_channels<T, V>(a.bias, at.channel[m], C(0), b);
+                    fetch_weights(m, w, b);
                 }
             };
             if constexpr (!BACK) {
@@ -192,29 +198,40 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     one_by_one();
                 }
             } else {
-                const C mean = now.mean[u], rstd = now.rstd[u];
+                const C rstd = now.rstd[u];
                 C hat[M][V], wd[M][V];
                 C wd_sum = 0, wdh_sum = 0;
+                // A row that is not there adds nothing, whatever its channels' weights would make of zeros; nor does a
+                // vector without elements: its elements, mean, weights and gradients are zero.
+                if (!now.on[u]) {
 #pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    C w[V], b[V], z[V];
-                    weights(m, w, b);
+                    for (int m = 0; m < M; ++m) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        hat[m][i] = (x[u][m].get(i) - mean) * rstd;
-                        z[i] = fma_(hat[m][i], w[i], b[i]);
+                        for (int i = 0; i < V; ++i) hat[m][i] = wd[m][i] = 0;
                     }
-                    slope_all<V>(s.activation, z);
-                    C part = 0, part_h = 0;
+                } else {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const C d = now.dy[u][m].get(i) * z[i];  // a lane without elements has zero gradients
-                        sum_d[m][i] += d, sum_dh[m][i] = fma_(d, hat[m][i], sum_dh[m][i]);
-                        wd[m][i] = w[i] * d;
-                        part += wd[m][i], part_h = fma_(wd[m][i], hat[m][i], part_h);
+                    for (int m = 0; m < M; ++m) {
+                        C w[V], b[V], z[V];
+                        weights(m, w, b);
+                        const C mean = at.on[m] ? now.mean[u] : C(0);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            hat[m][i] = (x[u][m].get(i) - mean) * rstd;
+                            z[i] = fma_(hat[m][i], w[i], b[i]);
+                        }
+                        slope_all<V>(s.activation, z);
+                        C part = 0, part_h = 0;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const C d = now.dy[u][m].get(i) * z[i];  // a lane without elements has zero gradients
+                            sum_d[m][i] += d, sum_dh[m][i] = fma_(d, hat[m][i], sum_dh[m][i]);
+                            wd[m][i] = w[i] * d;
+                            part += wd[m][i], part_h = fma_(wd[m][i], hat[m][i], part_h);
+                        }
+                        wd_sum += part, wdh_sum += part_h;
+                        one_by_one();
                     }
-                    wd_sum += part, wdh_sum += part_h;
-                    one_by_one();
                 }
                 group_sums(wd_sum, wdh_sum);
                 const C d_mean = wd_sum * static_cast<C>(share), dh_mean = wdh_sum * static_cast<C>(share);
