@@ -5,9 +5,11 @@ namespace hmr {
 namespace nn {
 namespace {
 
-// What is known of a set of elements: in f64 the sum and the sum of squares, which keep the variance's digits for 16- and
-// 32-bit elements with means up to 2^12 deviations from zero; for F64 the mean and the squares about it, joined pairwise,
-// of the elements less the group's first one (a mean far from zero would take its digits from the joins' differences).
+// What is known of a set of a group's elements. 16-bit ones: in f64 the sum and the sum of squares, which are exact where
+// their bits matter (elements within a few binades of a mean far from zero, up to 2^31 of them); the variance is their
+// difference with the products' rounding errors. F32: the same sums of the elements less the group's first one, from which
+// the mean of m elements is at most sqrt(m) deviations away, so that the variance is off by some m 2^-53 of itself. F64: the
+// mean and the squares about it of the elements less the first one, joined pairwise.
 template <class T>
 struct Moments {
     double n, a, b;
@@ -21,19 +23,24 @@ struct Moments {
             n = all;
         }
     }
-    __device__ __forceinline__ double mean(double less) const { return std::is_same_v<T, double> ? less + a : a / n; }
+    __device__ __forceinline__ double mean(double less) const { return less + (std::is_same_v<T, double> ? a : a / n); }
     __device__ __forceinline__ double variance() const {
         if constexpr (std::is_same_v<T, double>) return b / n;
-        const double m = a / n, v = __builtin_fma(-m, m, b / n);
+        const double squares = n * b, square = a * a;
+        const double v = ((squares - square) + (__builtin_fma(n, b, -squares) - __builtin_fma(a, a, -square))) / (n * n);
         return v < 0 ? 0 : v;
     }
 };
 
-// What a group's elements are taken less.
+// What a group's elements are taken less: 16-bit ones nothing, others the first one, unless that is infinite or NaN (the
+// mean then is).
 template <class T>
 __device__ __forceinline__ double less_of(const NormArgs &a, int64_t n, int64_t g) {
-    if constexpr (std::is_same_v<T, double>) return reinterpret_cast<const double *>(a.src.p)[n * a.src.sn + g * a.W];
-    else return 0;
+    if constexpr (sizeof(T) == 2) return 0;
+    else {
+        const double first = static_cast<double>(reinterpret_cast<const T *>(a.src.p)[n * a.src.sn + g * a.W]);
+        return first - first == 0 ? first : 0;
+    }
 }
 
 struct MapsArgs {
@@ -122,17 +129,19 @@ __global__ void __launch_bounds__(kBlock) moments_kernel(MapsArgs m) {
     Walk<T, V, 1> walk(at, a, m.p, a.src, a.src);
     // Of each of the lane's channels. F64 sums about the first one that the lane meets.
     double n = 0, sum[V], squares[V], about[V], less[V];
+    int64_t g = at.c / a.W, in = at.c - g * a.W;  // the channel's group, and its place there
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         sum[i] = squares[i] = about[i] = 0;
-        less[i] = at.on ? less_of<T>(a, at.n, (at.c + i) / a.W) : 0;
+        less[i] = at.on ? less_of<T>(a, at.n, g) : 0;
+        if (++in == a.W) in = 0, ++g;
     }
     walk.run([&](int64_t, const Vec<T, V> &x) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             double v = x.get(i);
+            if constexpr (sizeof(T) > 2) v -= less[i];
             if constexpr (std::is_same_v<T, double>) {
-                v -= less[i];
                 if (n == 0) about[i] = v;
                 v -= about[i];
             }

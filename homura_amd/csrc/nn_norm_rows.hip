@@ -143,8 +143,9 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                 }
             };
             if constexpr (!BACK) {
-                // Lanes without elements hold zeros. In f64 the squares of 16- and 32-bit elements are exact and their sum
-                // keeps the variance's digits for means up to 2^20 deviations from zero; F64 sums squares about the mean.
+                // Lanes without elements hold zeros. In f64 the squares of 16- and 32-bit elements are exact, and the variance
+                // from their sum is off by some 2^-53 (mean / deviation)^2 of itself and the additions' share: up to 2^10
+                // deviations less than f32 holds. Groups farther out, as F64 ones always, sum squares about the mean too.
                 double sum = 0, squares = 0;
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                 group_sums(sum, squares);
                 const double mean = sum * share;
                 double variance;
-                if constexpr (std::is_same_v<T, double>) {
+                auto about_the_mean = [&] {
                     double centred = 0, none = 0;
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
@@ -168,12 +169,21 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                             const double v = x[u][m].get(i) - mean;
                             if (at.on[m]) centred = __builtin_fma(v, v, centred);
                         }
+                        one_by_one();
                     }
                     group_sums(centred, none);
-                    variance = centred * share;
+                    return centred * share;
+                };
+                if constexpr (std::is_same_v<T, double>) {
+                    variance = about_the_mean();
                 } else {
                     variance = __builtin_fma(-mean, mean, squares * share);
-                    variance = variance < 0 ? 0 : variance;
+                    // Each group by its own mean and variance, whatever else the wave holds (a wide one is the workgroup's).
+                    const bool far = mean * mean > 0x1p20 * variance;
+                    if (__any(far)) {
+                        const double centred = about_the_mean();
+                        variance = far ? centred : variance;
+                    }
                 }
                 const double rstd = reciprocal_root(variance + a.eps);
                 if (now.on[u] && slot_on && first == 0) {
