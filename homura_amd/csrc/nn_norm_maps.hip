@@ -95,8 +95,9 @@ struct Walk {
             }
         }
     }
-    template <class F>
-    __device__ __forceinline__ void run(F f) {
+    // Calls f for every position, and done() after every kAtOnce of them.
+    template <class F, class D>
+    __device__ __forceinline__ void run(F f, D done) {
         while (s < S) {
             Vec<T, V> now[MAPS][kAtOnce];
 #pragma unroll
@@ -114,7 +115,12 @@ struct Walk {
                     else f(here + k * slots, now[0][k]);
                 }
             }
+            done();
         }
+    }
+    template <class F>
+    __device__ __forceinline__ void run(F f) {
+        run(f, [] {});
     }
 };
 
@@ -296,9 +302,14 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
     const NormArgs &a = m.a;
     const Place<V> at(a, m.p);
     Walk<T, V, 2> walk(at, a, m.p, a.src, a.grad);
-    C sum[V], sum_h[V];
+    constexpr bool kRuns = sizeof(C) == 4;
+    C sum[V], sum_h[V], all[kRuns ? V : 1], all_h[kRuns ? V : 1];
+    int run = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = sum_h[i] = 0;
+    for (int i = 0; i < V; ++i) {
+        sum[i] = sum_h[i] = 0;
+        if constexpr (kRuns) all[i] = all_h[i] = 0;
+    }
     if (at.on) {
         C w[V], b[V], mean[V], rstd[V];
         load_channels<T, V>(a.weight, at.c, C(1), w);
@@ -312,11 +323,23 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
                 const C d = dy.get(i) * z[i];
                 sum[i] += d, sum_h[i] = fma_(d, hat[i], sum_h[i]);
             }
+        }, [&] {
+            if constexpr (kRuns) {
+                run += kAtOnce;
+                if (run == kMostRun) {
+                    run = 0;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) add_run(all[i], sum[i]), add_run(all_h[i], sum_h[i]);
+                }
+            }
         });
     }
     __shared__ C slots[2][kBlock][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) slots[0][threadIdx.x][i] = sum_h[i], slots[1][threadIdx.x][i] = sum[i];
+    for (int i = 0; i < V; ++i) {
+        if constexpr (kRuns) sum[i] += all[i], sum_h[i] += all_h[i];
+        slots[0][threadIdx.x][i] = sum_h[i], slots[1][threadIdx.x][i] = sum[i];
+    }
     __syncthreads();
     C *out = static_cast<C *>(m.room);
     const int64_t rows = a.N * m.p.chunks, part = at.n * m.p.chunks + at.chunk;

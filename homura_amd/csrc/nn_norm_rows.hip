@@ -84,14 +84,28 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
         if constexpr (M > 2) __builtin_amdgcn_sched_barrier(0);
     };
     const double share = 1.0 / (static_cast<double>(a.S) * static_cast<double>(a.W));
-    C sum_d[BACK ? M : 1][V], sum_dh[BACK ? M : 1][V];
+    // The lane's sums of d and d * hat over its rows, in f32 by runs.
+    constexpr bool kRuns = BACK && sizeof(C) == 4;
+    C sum_d[BACK ? M : 1][V], sum_dh[BACK ? M : 1][V], all_d[kRuns ? M : 1][V], all_dh[kRuns ? M : 1][V];
+    int run = 0;
     if constexpr (BACK) {
 #pragma unroll
         for (int m = 0; m < M; ++m) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum_d[m][i] = sum_dh[m][i] = 0;
+            for (int i = 0; i < V; ++i) {
+                sum_d[m][i] = sum_dh[m][i] = 0;
+                if constexpr (kRuns) all_d[m][i] = all_dh[m][i] = 0;
+            }
         }
     }
+    auto end_run = [&] {
+        run = 0;
+#pragma unroll
+        for (int m = 0; m < (kRuns ? M : 0); ++m) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) add_run(all_d[m][i], sum_d[m][i]), add_run(all_dh[m][i], sum_dh[m][i]);
+        }
+    };
     // The next rows are under way while these are worked on.
     struct Rows {
         Vec<T, V> x[U][M], dy[BACK ? U : 1][M];
@@ -256,9 +270,19 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                 }
             }
         }
+        if constexpr (kRuns) {
+            if (++run == kMostRun) end_run();
+        }
     }
     if constexpr (BACK) {
         if (!s.weights) return;
+        if constexpr (kRuns) {
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum_d[m][i] += all_d[m][i], sum_dh[m][i] += all_dh[m][i];
+            }
+        }
         // The lanes of one channel (a lane of every wave; of several positions and rows where those are side by side) are
         // added in order by the thread that owns the channel in the workgroup's block.
         constexpr int kSpread = WIDE ? kBlock : 64;
