@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
         for (int64_t i = threadIdx.x; i < m; i += kBlock) {
             const int64_t s = i / a.W, c = c0 + i % a.W;
             const C hat = static_cast<C>((Comp<T>::up(a.src.get<T>(n, s, c)) - mean) * rstd);
-            a.out.put<T>(n, s, c, Comp<T>::down(activate<ACT>(hat * weight_of<T>(a.weight, c) + bias_of<T>(a.bias, c))));
+            a.out.put<T>(n, s, c, Comp<T>::down(activate<T, ACT>(hat * weight_of<T>(a.weight, c) + bias_of<T>(a.bias, c))));
         }
     }
 }
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kBlock) norm_back_kernel(NormArgs a) {
             const int64_t s = i / a.W, c = c0 + i % a.W;
             const C w = weight_of<T>(a.weight, c);
             hat = (Comp<T>::up(a.src.get<T>(n, s, c)) - mean) * rstd;
-            d = w * Comp<T>::up(a.grad.get<T>(n, s, c)) * slope<ACT>(hat * w + bias_of<T>(a.bias, c));
+            d = w * Comp<T>::up(a.grad.get<T>(n, s, c)) * slope<T, ACT>(hat * w + bias_of<T>(a.bias, c));
         };
         double d_sum = 0, dh_sum = 0;
         for (int64_t i = threadIdx.x; i < m; i += kBlock) {
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kBlock) norm_weights_kernel(NormArgs a) {
             const int64_t n = i / a.S, s = i - n * a.S, g = c / a.W;
             const C mean = reinterpret_cast<const C *>(a.mean.p)[a.mean.at(n, g)], rstd = reinterpret_cast<const C *>(a.rstd.p)[a.rstd.at(n, g)];
             const C hat = (Comp<T>::up(a.src.get<T>(n, s, c)) - mean) * rstd;
-            const C d = Comp<T>::up(a.grad.get<T>(n, s, c)) * slope<ACT>(hat * w + b);
+            const C d = Comp<T>::up(a.grad.get<T>(n, s, c)) * slope<T, ACT>(hat * w + b);
             d_sum += d, dh_sum += static_cast<double>(d) * hat;
         }
         d_sum = workgroup_sum(d_sum), dh_sum = workgroup_sum(dh_sum);

@@ -45,10 +45,15 @@ struct NormArgs {
 
 // ---- activations in the computation type -------------------------------------------------------------------------
 
-// 1 / (1 + exp(-z)) of an f32 from the hardware's exp2 and reciprocal, within three units of its last place.
+// 1 / (1 + exp(-z)) of an f32 from the hardware's exp2 and reciprocal, within seven half steps, beside 16-bit tensors |z| more
+// where z is negative (exp_parts; below 2^-126 it is zero). Where exp(-z) is past f32, e is infinite and 1 + t is not zero.
+template <class T>
 __device__ __forceinline__ float logistic(float z) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+    float e, t;
+    exp_parts<T>(-z, e, t);
+    return __builtin_amdgcn_rcpf(sizeof(T) > 2 ? fma_(e, 1.0f + t, 1.0f) : 1.0f + e);
 }
+template <class T>
 __device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-z)); }
 
 constexpr double kRootHalf = 0.70710678118654752440;       // sqrt(1/2)
@@ -56,9 +61,9 @@ constexpr double kRootTwoByPi = 0.79788456080286535588;    // sqrt(2/pi)
 constexpr double kTanhInner = 0.044715;
 
 // (1 + tanh(u)) / 2 is the logistic function of 2 u, which keeps its digits where tanh nears -1.
-template <class C>
+template <class T, class C>
 __device__ __forceinline__ C tanh_gate(C z) {
-    return logistic(z * fma_(C(2 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)));
+    return logistic<T>(z * fma_(C(2 * kRootTwoByPi * kTanhInner) * z, z, C(2 * kRootTwoByPi)));
 }
 
 // The normal distribution below z, and exp(-z^2 / 2). With a = |z| the tail beyond a is exp(-a^2 / 2) E(a), and E, which
@@ -81,36 +86,36 @@ __device__ __forceinline__ void normal(double z, double &below, double &bell) {
     below = 0.5 * erfc(-z * kRootHalf), bell = exp(-0.5 * z * z);
 }
 
-template <int ACT, class C>
+template <class T, int ACT, class C>
 __device__ __forceinline__ C activate(C z) {
     if constexpr (ACT == HMR_UNARY_RELU) {
         return z < C(0) ? C(0) : z;
     } else if constexpr (ACT == HMR_UNARY_SILU) {
-        return z * logistic(z);
+        return z * logistic<T>(z);
     } else if constexpr (ACT == HMR_UNARY_GELU) {
         C below, bell;
         normal(z, below, bell);
         return z * below;
     } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
-        return z * tanh_gate(z);
+        return z * tanh_gate<T>(z);
     } else {
         return z;
     }
 }
 
-template <int ACT, class C>
+template <class T, int ACT, class C>
 __device__ __forceinline__ C slope(C z) {
     if constexpr (ACT == HMR_UNARY_RELU) {
         return z > C(0) ? C(1) : (z != z ? z : C(0));
     } else if constexpr (ACT == HMR_UNARY_SILU) {
-        const C q = logistic(z);
+        const C q = logistic<T>(z);
         return fma_(z * q, C(1) - q, q);
     } else if constexpr (ACT == HMR_UNARY_GELU) {
         C below, bell;
         normal(z, below, bell);
         return fma_(z * bell, C(0.5 * kRootTwoByPi), below);
     } else if constexpr (ACT == HMR_UNARY_GELU_TANH) {
-        const C q = tanh_gate(z);
+        const C q = tanh_gate<T>(z);
         // Far out, where q (1 - q) is zero, z^2 is kept finite.
         return fma_(z * q * (C(1) - q), fma_(C(6 * kRootTwoByPi * kTanhInner), fmin(z * z, C(1e30)), C(2 * kRootTwoByPi)), q);
     } else {
@@ -143,23 +148,23 @@ __host__ __device__ __forceinline__ bool with_activation(int32_t activation, F &
     }
 }
 // The same choice on the device, once for V elements (the activation is the launch's, so that nothing diverges).
-template <int V, class C>
+template <class T, int V, class C>
 __device__ __forceinline__ void activate_all(int32_t activation, C (&z)[V]) {
     with_activation(activation, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            z[i] = activate<decltype(act)::value>(z[i]);
+            z[i] = activate<T, decltype(act)::value>(z[i]);
             // The 64-bit error function's many intermediate values, of one element at a time.
             if constexpr (decltype(act)::value == HMR_UNARY_GELU && sizeof(C) == 8) __builtin_amdgcn_sched_barrier(0);
         }
     });
 }
-template <int V, class C>
+template <class T, int V, class C>
 __device__ __forceinline__ void slope_all(int32_t activation, C (&z)[V]) {
     with_activation(activation, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            z[i] = slope<decltype(act)::value>(z[i]);
+            z[i] = slope<T, decltype(act)::value>(z[i]);
             // The 64-bit error function's many intermediate values, of one element at a time.
             if constexpr (decltype(act)::value == HMR_UNARY_GELU && sizeof(C) == 8) __builtin_amdgcn_sched_barrier(0);
         }

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(MapsArgs m, const double 
         C z[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) z[i] = fma_(x.get(i) - near[i], w[i], b[i]);
-        activate_all<V>(m.activation, z);
+        activate_all<T, V>(m.activation, z);
         Vec<T, V> y;
         y.round(z);
         y.template store<PAST>(to + s * a.out.ss);
@@ -284,7 +284,7 @@ __device__ __forceinline__ void hat_and_slope(int32_t activation, const Vec<T, V
         hat[i] = (x.get(i) - mean[i]) * rstd[i];
         z[i] = fma_(hat[i], w[i], b[i]);
     }
-    slope_all<V>(activation, z);
+    slope_all<T, V>(activation, z);
 }
 template <class T, int V, class C>
 __device__ __forceinline__ void load_statistics(const NormArgs &a, int64_t n, int64_t c, C (&mean)[V], C (&rstd)[V]) {

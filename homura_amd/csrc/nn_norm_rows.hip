@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                     weights(m, w, b);
 #pragma unroll
                     for (int i = 0; i < V; ++i) z[i] = fma_(centre.hat(x[u][m].get(i)), w[i], b[i]);
-                    activate_all<V>(s.activation, z);
+                    activate_all<T, V>(s.activation, z);
                     Vec<T, V> y;
                     y.round(z);
                     if (now.on[u] && at.on[m]) y.template store<PAST>(reinterpret_cast<T *>(a.out.p) + n[u] * a.out.sn + at.out[m]);
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
                             hat[m][i] = (x[u][m].get(i) - mean) * rstd;
                             z[i] = fma_(hat[m][i], w[i], b[i]);
                         }
-                        slope_all<V>(s.activation, z);
+                        slope_all<T, V>(s.activation, z);
                         C part = 0, part_h = 0;
 #pragma unroll
                         for (int i = 0; i < V; ++i) {

@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(kBlock) forward_kernel(RecurrenceArgs a) {
         for (int64_t t = 0; t < a.T; ++t) {
             C f, u, y = 0;
             if (t < steps) {
-                factor_and_input<FORM>(Comp<T>::up(a.gate.template get<T>(b, t, c)), Comp<T>::up(a.input.template get<T>(b, t, c)), f, u);
+                factor_and_input<T, FORM>(Comp<T>::up(a.gate.template get<T>(b, t, c)), Comp<T>::up(a.input.template get<T>(b, t, c)), f, u);
                 y = h = fma_(f, h, u);
             }
             a.out.template put<T>(b, t, c, Comp<T>::down(y));
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kBlock) backward_kernel(RecurrenceArgs a) {
                 C before = 0;
                 if (t > 0) before = Comp<T>::up(a.state.template get<T>(b, t - 1, c));
                 else if (a.initial.p != nullptr) before = load_state<T>(a.initial.p, a.initial.at(b, c), a.initial.wide);
-                e = step_back<FORM>(z, x, g, before, dg, dx);
+                e = step_back<T, FORM>(z, x, g, before, dg, dx);
             }
             a.d_gate.template put<T>(b, t, c, Comp<T>::down(dg));
             a.d_input.template put<T>(b, t, c, Comp<T>::down(dx));

@@ -50,13 +50,18 @@ struct RecurrenceArgs {
     }
 };
 
-// sigmoid(z) and 1 - sigmoid(z), each to within a few units of its own last place: the smaller of the two comes from
-// exp(-|z|) itself, not from a subtraction.
+// sigmoid(z) and 1 - sigmoid(z), each to within seven half steps of its own, |z| more for the smaller one beside 16-bit
+// sequences (exp_parts; below 2^-126 it is zero): the smaller of the two comes from exp(-|z|) itself, not from a subtraction.
+template <class T>
 __device__ __forceinline__ void sigmoid_pair(float z, float &a, float &rest) {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504088896341f * fabsf(z)), q = __builtin_amdgcn_rcpf(1.0f + e), r = e * q;
+    float e, t;
+    exp_parts<T>(-fabsf(z), e, t);
+    if constexpr (sizeof(T) > 2) e = fma_(e, t, e);
+    const float q = __builtin_amdgcn_rcpf(1.0f + e), r = e * q;
     a = z < 0.0f ? r : q;
     rest = z < 0.0f ? q : r;
 }
+template <class T>
 __device__ __forceinline__ void sigmoid_pair(double z, double &a, double &rest) {
     const double e = exp(-fabs(z)), q = 1.0 / (1.0 + e), r = e * q;
     a = z < 0.0 ? r : q;
@@ -64,27 +69,27 @@ __device__ __forceinline__ void sigmoid_pair(double z, double &a, double &rest) 
 }
 
 // The factor and the addend of a step.
-template <int FORM, class C>
+template <class T, int FORM, class C>
 __device__ __forceinline__ void factor_and_input(C gate, C input, C &factor, C &addend) {
     if constexpr (FORM == HMN_GATE_FACTOR) {
         factor = gate, addend = input;
     } else {
         C rest;
-        sigmoid_pair(gate, factor, rest);
+        sigmoid_pair<T>(gate, factor, rest);
         addend = rest * input;
     }
 }
 
 // A step backwards: from the gradient g of the state it led to, the gradients of its gate and input and what is handed
 // back to the state before it.
-template <int FORM, class C>
+template <class T, int FORM, class C>
 __device__ __forceinline__ C step_back(C gate, C input, C g, C before, C &d_gate, C &d_input) {
     if constexpr (FORM == HMN_GATE_FACTOR) {
         d_gate = g * before, d_input = g;
         return gate * g;
     } else {
         C a, rest;
-        sigmoid_pair(gate, a, rest);
+        sigmoid_pair<T>(gate, a, rest);
         const C back = a * g;
         d_input = rest * g;
         d_gate = (before - input) * (back * rest);

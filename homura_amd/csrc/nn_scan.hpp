@@ -184,10 +184,10 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     auto map = [&](int i, int j, C &f, C &add) {
         const C z = now.gate[i].get(j);
         if constexpr (!BACK) {
-            factor_and_input<FORM>(z, now.input[i].get(j), f, add);
+            factor_and_input<T, FORM>(z, now.input[i].get(j), f, add);
         } else {
             C rest;
-            if constexpr (FORM == HMN_GATE_SIGMOID) sigmoid_pair(z, f, rest);
+            if constexpr (FORM == HMN_GATE_SIGMOID) sigmoid_pair<T>(z, f, rest);
             else f = z;
             add = f * now.grad[i].get(j);
         }
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
                     const C g = now.grad[i].get(j) + e[j];
                     C x = 0;
                     if constexpr (FORM == HMN_GATE_SIGMOID) x = now.input[i].get(j);
-                    e[j] = step_back<FORM>(now.gate[i].get(j), x, g, before, dg[j], dx[j]);
+                    e[j] = step_back<T, FORM>(now.gate[i].get(j), x, g, before, dg[j], dx[j]);
                 }
                 out.round(dg);
                 out.only(t.has(i));
