@@ -72,10 +72,10 @@ __device__ __forceinline__ double fma_(double a, double b, double c) { return __
 
 // exp(v) in two parts, e and t: exp(v) = e (1 + t). e is the hardware's exp2 of the nearest f32 to v log2(e), and t what that
 // rounding left of v. With it the exponential is off by some three half steps, without it by up to |v| more. Beside 16-bit
-// tensors t is zero: |v| is below 104 where the result is not zero, and so many half steps of f32 are a 20th of the half step
-// that such a tensor rounds by; the corrected form takes longer: sigmoid over [8, 2048, 4096] bf16 120 us for 108, norm + silu
-// over [16384, 4096] 71 for 64; in f32 [2, 16411, 1003] 99.5 for 97. Where the product is infinite, t (which is then NaN or infinite) is at most 1, and e
-// zero or infinity. e is zero where it would be below 2^-126.
+// tensors t is zero: |v| is below 104 where the result is not zero, and so many half steps of f32 are less than a 70th of the
+// half step that such a tensor rounds by; the corrected form takes longer: sigmoid over [8, 2048, 4096] bf16 120 us for 108,
+// norm + silu over [16384, 4096] 71 for 64; in f32 [2, 16411, 1003] 99.5 for 97. Where the product is infinite, t (which is
+// then NaN or infinite) is at most 1, and e zero or infinity. e is zero where it would be below 2^-126.
 template <class T>
 __device__ __forceinline__ void exp_parts(float v, float &e, float &t) {
     constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f, kLn2Rest = -1.90465429995776804e-9f;

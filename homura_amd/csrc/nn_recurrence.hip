@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kBlock) backward_kernel(RecurrenceArgs a) {
                 else if (a.initial.p != nullptr) before = load_state<T>(a.initial.p, a.initial.at(b, c), a.initial.wide);
                 e = step_back<T, FORM>(z, x, g, before, dg, dx);
             }
-            a.d_gate.template put<T>(b, t, c, Comp<T>::down(dg));
+            store_state<T>(a.d_gate.p, a.d_gate.at(b, t, c), a.d_gate_wide, dg);
             a.d_input.template put<T>(b, t, c, Comp<T>::down(dx));
         }
         if (a.exit.p != nullptr) store_state<T>(a.exit.p, a.exit.at(b, c), a.exit.wide, e);
@@ -165,15 +165,16 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
     // The factor form's gradients do not need its input.
     if (form == HMN_GATE_FACTOR && input == nullptr) input = gate;
     if (hmr_status s = check_batch(who, form, gate,
-                                   {{"d_gate", d_gate, true}, {"d_input", d_input, true}, {"grad", grad, false},
-                                    {"input", input, false}, {"out", out, false}},
+                                   {{"d_input", d_input, true}, {"grad", grad, false}, {"input", input, false}, {"out", out, false}},
                                    {{"d_initial", d_initial, true}, {"grad_last", grad_last, false}, {"initial", initial, false}},
                                    lengths)) {
         return s;
     }
+    if (hmr_status s = check_operand(who, "d_gate", d_gate, 3, gate->sizes, true)) return s;
+    if (hmr_status s = check_type(who, "d_gate", d_gate->dtype, gate->dtype, wide_type(gate->dtype))) return s;
     RecurrenceArgs a = batch_args(gate, lengths);
     a.input = sequences_of(input), a.grad = sequences_of(grad), a.state = sequences_of(out);
-    a.d_gate = sequences_of(d_gate), a.d_input = sequences_of(d_input);
+    a.d_gate = sequences_of(d_gate), a.d_gate_wide = d_gate->dtype == HMR_F32, a.d_input = sequences_of(d_input);
     a.entry = states_of(grad_last), a.exit = states_of(d_initial), a.initial = states_of(initial);
     if (hmr_status s = check_room(who, workspace, workspace_bytes, room_for(gate))) return s;
     if (ctx == nullptr) return refuse(who, "null context");

@@ -35,6 +35,7 @@ struct RecurrenceArgs {
     int64_t B, T, C;
     Sequences gate, input, out;                // forwards
     Sequences grad, state, d_gate, d_input;    // backwards, with gate and input
+    bool d_gate_wide;                          // f32 beside 16-bit sequences
     States entry, exit;                        // initial and last; grad_last and d_initial
     States initial;                            // backwards
     const char *lengths;                       // or nullptr

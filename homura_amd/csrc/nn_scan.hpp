@@ -136,16 +136,17 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     // The address of a tile's earliest step (less `back`) and first channel, the same for the whole workgroup, and the
     // lane's offset from there to its own earliest step in 32 bits (the host has checked that a tile spans less); step i
     // of the lane is a number of steps on that is the same for the whole workgroup again.
-    auto base = [&](const Tile &t, const Sequences &x, int back = 0) {
+    auto base_of = [&](const Tile &t, const Sequences &x, int back, int64_t size) {
         const int64_t first = BACK ? a.T - (t.k + 1) * TT : t.k * TT;
-        return x.p + (t.b * x.sb + (first - back) * x.st + t.c0 * x.sc) * static_cast<int64_t>(sizeof(T));
+        return x.p + (t.b * x.sb + (first - back) * x.st + t.c0 * x.sc) * size;
     };
-    auto row = [&](char *from, const Tile &t, const Sequences &x, int i) {
+    auto row_of = [&](char *from, const Tile &t, const Sequences &x, int i, uint32_t size) {
         const int lane_step = BACK ? TT - S - r * S : r * S, step = BACK ? S - 1 - i : i;
-        const uint32_t off = (static_cast<uint32_t>(lane_step) * static_cast<uint32_t>(x.st) + static_cast<uint32_t>(t.at) * static_cast<uint32_t>(x.sc)) *
-                             static_cast<uint32_t>(sizeof(T));
-        return reinterpret_cast<T *>(from + step * x.st * static_cast<int64_t>(sizeof(T)) + off);
+        const uint32_t off = (static_cast<uint32_t>(lane_step) * static_cast<uint32_t>(x.st) + static_cast<uint32_t>(t.at) * static_cast<uint32_t>(x.sc)) * size;
+        return from + step * x.st * static_cast<int64_t>(size) + off;
     };
+    auto base = [&](const Tile &t, const Sequences &x, int back = 0) { return base_of(t, x, back, sizeof(T)); };
+    auto row = [&](char *from, const Tile &t, const Sequences &x, int i) { return reinterpret_cast<T *>(row_of(from, t, x, i, sizeof(T))); };
     // Steps outside the sequence get what maps a value to itself: a factor of one (sigmoid's at infinity) and nothing to add.
     auto load = [&](const Tile &t, Raw &raw) {
         char *gate = base(t, a.gate), *input = nullptr, *grad = nullptr, *before = nullptr;
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
 #pragma unroll
     for (int j = 0; j < V; ++j) e[j] = t.lane_on ? slot_u[r][t.at + j] : C(0);
     if (t.lane_on) {
-        char *const to = base(t, BACK ? a.d_gate : a.out), *const to_input = BACK ? base(t, a.d_input) : nullptr;
+        char *const to = BACK && sizeof(T) < sizeof(C) && a.d_gate_wide ? base_of(t, a.d_gate, 0, sizeof(C)) : base(t, BACK ? a.d_gate : a.out), *const to_input = BACK ? base(t, a.d_input) : nullptr;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             Vec<T, V> out;
@@ -324,9 +325,16 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
                     if constexpr (FORM == HMN_GATE_SIGMOID) x = now.input[i].get(j);
                     e[j] = step_back<T, FORM>(now.gate[i].get(j), x, g, before, dg[j], dx[j]);
                 }
-                out.round(dg);
-                out.only(t.has(i));
-                if (i < t.end) out.template store<kStorePast>(row(to, t, a.d_gate, i));
+                if (sizeof(T) < sizeof(C) && a.d_gate_wide) {
+                    Vec<C, V> wide;
+                    wide.round(dg);
+                    wide.only(t.has(i));
+                    if (i < t.end) wide.template store<kStorePast>(reinterpret_cast<C *>(row_of(to, t, a.d_gate, i, sizeof(C))));
+                } else {
+                    out.round(dg);
+                    out.only(t.has(i));
+                    if (i < t.end) out.template store<kStorePast>(row(to, t, a.d_gate, i));
+                }
                 out.round(dx);
                 out.only(t.has(i));
                 if (i < t.end) out.template store<kStorePast>(row(to_input, t, a.d_input, i));

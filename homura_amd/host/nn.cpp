@@ -142,14 +142,18 @@ Recurrence linear_recurrence(const std::optional<Tensor> &g, const std::optional
         expect_dtype(op, "the last state's gradient", *g_last, input.dtype(), wide(input.dtype()));
     }
     const Tensor dy = g ? *g : Tensor::full({1}, Scalar::of_float(0.0), input.dtype(), input.device()).expand(as_spec(b.shape));
-    Tensor d_gate = Tensor::uninit_on({b.B, b.T, b.C}, input.dtype(), input.device());
+    // A gate that was broadcast gets the sum of many gradients, which are rounded to its type once, after that.
+    const bool shared = gate.shape() != b.shape;
+    Tensor d_gate = Tensor::uninit_on({b.B, b.T, b.C}, shared ? wide(input.dtype()) : input.dtype(), input.device());
     Tensor d_input = Tensor::uninit_on({b.B, b.T, b.C}, input.dtype(), input.device());
     Tensor d_initial = Tensor::uninit_on({b.B, b.C}, initial ? initial->dtype() : wide(input.dtype()), input.device());
     const std::optional<Tensor> from = b.state(initial), from_last = b.state(g_last);
     backend::recurrence_backward(sigmoid, d_gate.data(), d_input.data(), d_initial.data(), b.sequences(dy).data(), data(from_last),
                                  b.sequences(gate.expand(as_spec(b.shape))).data(), b.sequences(input).data(), b.sequences(out).data(),
                                  data(from), data(lengths));
-    return {d_gate.reshape(as_spec(b.shape)).sum_to_size(gate.shape()), d_input.reshape(as_spec(b.shape)), d_initial.reshape(as_spec(b.states))};
+    d_gate = d_gate.reshape(as_spec(b.shape));
+    if (shared) d_gate = d_gate.sum_to_size(gate.shape()).to(input.dtype());
+    return {d_gate, d_input.reshape(as_spec(b.shape)), d_initial.reshape(as_spec(b.states))};
 }
 
 }  // namespace grad

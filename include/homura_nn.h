@@ -66,7 +66,8 @@ hmr_status hmn_recurrence(hmr_context_t ctx, int32_t form, const hmr_tensor_desc
  *   GATE_FACTOR    d_input = g_t,             d_gate = g_t * h_{t-1}
  *   GATE_SIGMOID   d_input = (1 - a_t) g_t,   d_gate = g_t * (h_{t-1} - input_t) * a_t * (1 - a_t)
  * and d_initial = a_1 g_1. `grad_last`, `initial` and `d_initial` may be NULL (zero, zero, not wanted); the three states
- * may be F32 beside F16 or BF16 sequences. Behind a sequence's length d_gate and d_input are zero and `grad` is not
+ * may be F32 beside F16 or BF16 sequences, and so may `d_gate` (where one gate serves many channels or sequences, so that
+ * their gradients are summed before they are rounded). Behind a sequence's length d_gate and d_input are zero and `grad` is not
  * read. d_initial may be grad_last itself.
  */
 hmr_status hmn_recurrence_backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_gate,
