@@ -175,7 +175,8 @@ hmr_status forward(hmr_context_t ctx, const hmr_tensor_desc *out, const hmr_tens
     NormArgs a = norm_args(src, groups);
     a.out = maps_of(out), a.mean = per_group(mean), a.rstd = per_group(rstd);
     a.weight = per_channel(weight), a.bias = per_channel(bias), a.eps = eps;
-    if (a.N == 0 || a.C == 0) return HMR_OK;
+    // Without positions there are only the statistics to write.
+    if (a.N == 0 || a.C == 0 || (a.S == 0 && a.mean.p == nullptr && a.rstd.p == nullptr)) return HMR_OK;
     return queue_on(ctx, who, [&](hipStream_t stream) {
         if (queue_norm_rows(stream, src->dtype, a, activation, workspace, false)) return true;
         if (queue_norm_maps(stream, src->dtype, a, activation, workspace, false)) return true;

@@ -125,6 +125,9 @@ bool near_by(std::initializer_list<const hmr_tensor_desc *> operands) {
     return true;
 }
 
+// Without a step there is only the state to hand over; without anyone who wants it nothing, however many sequences there are.
+bool nothing_to_write(const RecurrenceArgs &a) { return a.B == 0 || a.C == 0 || (a.T == 0 && a.exit.p == nullptr); }
+
 uint32_t grid_of(hmr_context_t ctx, const RecurrenceArgs &a) {
     const int64_t groups = (a.B * a.C + kBlock - 1) / kBlock, most = int64_t{64} * ctx->compute_units;
     return static_cast<uint32_t>(groups < most ? groups : most);
@@ -142,7 +145,7 @@ hmr_status forward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *out, 
     a.input = sequences_of(input), a.out = sequences_of(out), a.entry = states_of(initial), a.exit = states_of(last);
     if (hmr_status s = check_room(who, workspace, workspace_bytes, room_for(gate))) return s;
     if (ctx == nullptr) return refuse(who, "null context");
-    if (a.B * a.C == 0) return HMR_OK;
+    if (nothing_to_write(a)) return HMR_OK;
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
@@ -178,7 +181,7 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
     a.entry = states_of(grad_last), a.exit = states_of(d_initial), a.initial = states_of(initial);
     if (hmr_status s = check_room(who, workspace, workspace_bytes, room_for(gate))) return s;
     if (ctx == nullptr) return refuse(who, "null context");
-    if (a.B * a.C == 0) return HMR_OK;
+    if (nothing_to_write(a)) return HMR_OK;
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
