@@ -132,10 +132,13 @@ struct ScanShape {
     static constexpr int kV = V, kR = R, kS = S, kLanes = kScanBlock / R, kChannels = kLanes * V, kSteps = R * S;
     static constexpr int kWords = sizeof(typename Comp<T>::C) / 4;  // 64-bit words of an entry
 
+    static int64_t blocks(int64_t C) { return C / kChannels + (C % kChannels != 0); }
+    static int64_t tiles(int64_t steps) { return steps / kSteps + (steps % kSteps != 0); }
+    // For no more tiles than a launch has workgroups.
     static ScanPlan plan(int64_t steps, int64_t C) {
         ScanPlan p{};
-        p.blocks = (C + kChannels - 1) / kChannels;
-        p.tiles = (steps + kSteps - 1) / kSteps;
+        p.blocks = blocks(C);
+        p.tiles = tiles(steps);
         p.group = 1;
         while (p.group * p.group < p.tiles) ++p.group;
         p.by_sequence = make_fastdiv(static_cast<uint32_t>(p.blocks * p.tiles)), p.by_blocks = make_fastdiv(static_cast<uint32_t>(p.blocks));

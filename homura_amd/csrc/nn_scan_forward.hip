@@ -10,13 +10,13 @@ void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const R
 
 namespace {
 
-// The most that any shape makes of measure(shape, its plan).
+// The most that any shape makes of measure(shape).
 template <class F>
 int64_t most_of(const hmr_tensor_desc *gate, F measure) {
     int64_t most = 0;
     with_float_type(gate->dtype, [&](auto tag) {
         with_scan_shapes<typename decltype(tag)::type>(gate->sizes[1], [&](auto shape) {
-            const int64_t x = measure(shape, decltype(shape)::plan(gate->sizes[1], gate->sizes[2]));
+            const int64_t x = measure(shape);
             if (x > most) most = x;
         });
     });
@@ -28,12 +28,20 @@ int64_t most_of(const hmr_tensor_desc *gate, F measure) {
 bool scan_used(const hmr_tensor_desc *gate) {
     if (gate->sizes[0] == 0 || gate->sizes[2] == 0 || gate->sizes[1] <= kFewSteps) return false;
     if (gate->sizes[1] <= kFewWithMany && gate->sizes[0] >= (kMany + gate->sizes[2] - 1) / gate->sizes[2]) return false;
-    return fits_launch(most_of(gate, [&](auto, const ScanPlan &p) { return gate->sizes[0] * p.blocks * p.tiles; }), kScanBlock);
+    return fits_launch(most_of(gate,
+                               [&](auto shape) {
+                                   using Shape = decltype(shape);
+                                   return gate->sizes[0] * Shape::blocks(gate->sizes[2]) * Shape::tiles(gate->sizes[1]);
+                               }),
+                       kScanBlock);
 }
 
 int64_t room_for(const hmr_tensor_desc *gate) {
     if (!scan_used(gate)) return 0;
-    return 8 * most_of(gate, [&](auto shape, const ScanPlan &p) { return decltype(shape)::words(p, gate->sizes[0]); });
+    return 8 * most_of(gate, [&](auto shape) {
+        using Shape = decltype(shape);
+        return Shape::words(Shape::plan(gate->sizes[1], gate->sizes[2]), gate->sizes[0]);
+    });
 }
 
 }  // namespace nn
