@@ -173,7 +173,14 @@ def load(path: str = LIB_PATH, prototypes=PROTOTYPES) -> ctypes.CDLL:
 
 
 lib = load()
-nn = load(NN_PATH, NN_PROTOTYPES)
+
+
+def __getattr__(name):
+    """`nn` is libhomura_nn.so, loaded when it is first asked for: without it, what needs libhomura_rocm.so alone works."""
+    if name != "nn":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()["nn"] = load(NN_PATH, NN_PROTOTYPES)
+    return globals()["nn"]
 
 
 def check(status: int) -> None:
@@ -184,7 +191,7 @@ def check(status: int) -> None:
 def check_nn(status: int) -> None:
     """check() for the calls of libhomura_nn, which keeps its own failure text."""
     if status != HMR_OK:
-        raise HmrError(status, nn.hmn_last_error().decode("utf-8", "replace"))
+        raise HmrError(status, __getattr__("nn").hmn_last_error().decode("utf-8", "replace"))
 
 
 def make_desc(ptr: int, dtype: int, sizes=(), strides=(), offset: int = 0) -> hmr_tensor_desc:

@@ -1,5 +1,7 @@
 // Storage, the device dispatch of every kernel, and the ROCm host side that turns tensors into
 // hmr_tensor_desc's and calls the C ABI. See homura.hpp for the map to the reference's files.
+#include <dlfcn.h>
+
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -1064,9 +1066,43 @@ std::optional<uint64_t> random_int_batch(const TensorData &out, uint64_t seed, u
 
 namespace {
 
+// The library is loaded by the first call that needs it, from beside this one: without it everything else runs.
+struct NnLibrary {
+    decltype(&hmn_last_error) last_error;
+    decltype(&hmn_recurrence_workspace) recurrence_workspace;
+    decltype(&hmn_recurrence) recurrence;
+    decltype(&hmn_recurrence_backward) recurrence_backward;
+    decltype(&hmn_group_norm_workspace) group_norm_workspace;
+    decltype(&hmn_group_norm) group_norm;
+    decltype(&hmn_group_norm_backward) group_norm_backward;
+    decltype(&hmn_dropout) dropout;
+
+    NnLibrary() {
+        void *library = dlopen("libhomura_nn.so", RTLD_NOW | RTLD_LOCAL);
+        if (!library) throw Error(std::string("libhomura_nn.so could not be loaded: ") + dlerror());
+        auto find = [&](auto &entry, const char *name) {
+            entry = reinterpret_cast<std::decay_t<decltype(entry)>>(dlsym(library, name));
+            if (!entry) throw Error(std::string("libhomura_nn.so has no ") + name);
+        };
+        find(last_error, "hmn_last_error");
+        find(recurrence_workspace, "hmn_recurrence_workspace");
+        find(recurrence, "hmn_recurrence");
+        find(recurrence_backward, "hmn_recurrence_backward");
+        find(group_norm_workspace, "hmn_group_norm_workspace");
+        find(group_norm, "hmn_group_norm");
+        find(group_norm_backward, "hmn_group_norm_backward");
+        find(dropout, "hmn_dropout");
+    }
+};
+
+const NnLibrary &nn() {
+    static const NnLibrary library;  // a failure is tried again by the next call
+    return library;
+}
+
 void expect_nn(hmr_status s) {
     if (s == HMR_OK) return;
-    std::string message = hmn_last_error();
+    std::string message = nn().last_error();
     if (s == HMR_OUT_OF_MEMORY) throw Error("ROCm out of memory: " + message);
     throw Error(message);
 }
@@ -1107,10 +1143,10 @@ void recurrence(bool sigmoid, const TensorData &out, const TensorData &last, con
     const hmr_tensor_desc o = whole_desc(out), l = whole_desc(last), g = whole_desc(gate), x = whole_desc(input);
     const MaybeDesc i(initial), n(lengths);
     int64_t bytes = 0;
-    expect_nn(hmn_recurrence_workspace(&g, &bytes));
+    expect_nn(nn().recurrence_workspace(&g, &bytes));
     auto ws = workspace(bytes, gate.device());
     exec(out, [&](hmr_context_t ctx) {
-        expect_nn(hmn_recurrence(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &o, &l, &g, &x, i.get(), n.get(),
+        expect_nn(nn().recurrence(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &o, &l, &g, &x, i.get(), n.get(),
                                  ws ? ws->ptr() : nullptr, bytes));
     });
 }
@@ -1122,10 +1158,10 @@ void recurrence_backward(bool sigmoid, const TensorData &d_gate, const TensorDat
     const hmr_tensor_desc z = whole_desc(gate), x = whole_desc(input), h = whole_desc(out);
     const MaybeDesc gl(g_last), i(initial), n(lengths);
     int64_t bytes = 0;
-    expect_nn(hmn_recurrence_workspace(&z, &bytes));
+    expect_nn(nn().recurrence_workspace(&z, &bytes));
     auto ws = workspace(bytes, gate.device());
     exec(out, [&](hmr_context_t ctx) {
-        expect_nn(hmn_recurrence_backward(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &dg, &dx, &di, &gr, gl.get(), &z, &x, &h,
+        expect_nn(nn().recurrence_backward(ctx, sigmoid ? HMN_GATE_SIGMOID : HMN_GATE_FACTOR, &dg, &dx, &di, &gr, gl.get(), &z, &x, &h,
                                           i.get(), n.get(), ws ? ws->ptr() : nullptr, bytes));
     });
 }
@@ -1135,10 +1171,10 @@ void group_norm(const TensorData &out, const TensorData &mean, const TensorData 
     const hmr_tensor_desc o = whole_desc(out), m = whole_desc(mean), r = whole_desc(rstd), s = whole_desc(src);
     const MaybeDesc w(weight), b(bias);
     int64_t bytes = 0;
-    expect_nn(hmn_group_norm_workspace(&s, groups, 0, &bytes));
+    expect_nn(nn().group_norm_workspace(&s, groups, 0, &bytes));
     auto ws = workspace(bytes, src.device());
     exec(out, [&](hmr_context_t ctx) {
-        expect_nn(hmn_group_norm(ctx, &o, &m, &r, &s, w.get(), b.get(), groups, eps, activation_code(activation),
+        expect_nn(nn().group_norm(ctx, &o, &m, &r, &s, w.get(), b.get(), groups, eps, activation_code(activation),
                                  ws ? ws->ptr() : nullptr, bytes));
     });
 }
@@ -1149,10 +1185,10 @@ void group_norm_backward(const TensorData &d_src, const TensorData *d_weight, co
     const hmr_tensor_desc ds = whole_desc(d_src), gr = whole_desc(g), s = whole_desc(src), m = whole_desc(mean), r = whole_desc(rstd);
     const MaybeDesc dw(d_weight), db(d_bias), w(weight), b(bias);
     int64_t bytes = 0;
-    expect_nn(hmn_group_norm_workspace(&s, groups, 1, &bytes));
+    expect_nn(nn().group_norm_workspace(&s, groups, 1, &bytes));
     auto ws = workspace(bytes, src.device());
     exec(d_src, [&](hmr_context_t ctx) {
-        expect_nn(hmn_group_norm_backward(ctx, &ds, dw.get(), db.get(), &gr, &s, &m, &r, w.get(), b.get(), groups,
+        expect_nn(nn().group_norm_backward(ctx, &ds, dw.get(), db.get(), &gr, &s, &m, &r, w.get(), b.get(), groups,
                                           activation_code(activation), ws ? ws->ptr() : nullptr, bytes));
     });
 }
@@ -1162,7 +1198,7 @@ void dropout(const TensorData &out, const TensorData &src, const TensorData *res
     if (residual) operands.push_back(residual);
     std::vector<hmr_tensor_desc> d;
     if (!descs("dropout", operands, d)) return;
-    exec(out, [&](hmr_context_t ctx) { expect_nn(hmn_dropout(ctx, &d[0], &d[1], residual ? &d[2] : nullptr, mask.p, mask.seed, mask.offset, nullptr)); });
+    exec(out, [&](hmr_context_t ctx) { expect_nn(nn().dropout(ctx, &d[0], &d[1], residual ? &d[2] : nullptr, mask.p, mask.seed, mask.offset, nullptr)); });
 }
 
 void upload(const TensorData &dst, const TensorData &src) {
