@@ -149,8 +149,9 @@ hmr_status forward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *out, 
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
-            if (scan_used(gate) && near_by({gate, input, out})) {
-                queue_scan_forward(stream, gate->dtype, form, a, layout_of({gate, input, out}), workspace);
+            const ScanLayout layout = layout_of({gate, input, out});
+            if ((scan_used(gate) || short_scan_used(gate, layout, false)) && near_by({gate, input, out})) {
+                queue_scan_forward(stream, gate->dtype, form, a, layout, workspace);
                 return;
             }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {
@@ -185,8 +186,9 @@ hmr_status backward(hmr_context_t ctx, int32_t form, const hmr_tensor_desc *d_ga
     return queue_on(ctx, who, [&](hipStream_t stream) {
         return with_float_type(gate->dtype, [&](auto tag) {
             using T = typename decltype(tag)::type;
-            if (scan_used(gate) && near_by({gate, input, out, grad, d_gate, d_input})) {
-                queue_scan_backward(stream, gate->dtype, form, a, layout_of({gate, input, out, grad, d_gate, d_input}), workspace);
+            const ScanLayout layout = layout_of({gate, input, out, grad, d_gate, d_input});
+            if ((scan_used(gate) || short_scan_used(gate, layout, true)) && near_by({gate, input, out, grad, d_gate, d_input})) {
+                queue_scan_backward(stream, gate->dtype, form, a, layout, workspace);
                 return;
             }
             with_code(form, std::integer_sequence<int, HMN_GATE_FACTOR, HMN_GATE_SIGMOID>{}, [&](auto f) {

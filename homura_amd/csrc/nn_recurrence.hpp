@@ -170,9 +170,15 @@ void queue_scan_forward(hipStream_t stream, int32_t dtype, int32_t form, const R
 void queue_scan_backward(hipStream_t stream, int32_t dtype, int32_t form, const RecurrenceArgs &a, const ScanLayout &layout, void *room);
 // Sequences of so few steps go a thread per channel: there is nothing to gain in a scan of up to eight ([64, 6, 4096] bf16
 // 5 us, 10 by a scan), nor of up to 32 where there are enough channels to keep the chip busy, 2^16 of all sequences
-// ([512, 24, 4096] bf16 97 us and 168, backwards 145 and 315; [4096, 16, 40] 7 and 19; but [512, 16, 4096] f32 84 and 71, and
-// [512, 64, 4096] bf16 248 and 186).
+// ([512, 24, 4096] bf16 95 us and 167, backwards 145 and 315; [4096, 16, 40] 7 and 18; but [512, 64, 4096] bf16 248 and 186).
 constexpr int64_t kFewSteps = 8, kFewWithMany = 32, kMany = int64_t{1} << 16;
+// Of those, 13 to 16 steps make a nearly full tile of the shortest shape, and where rows fill its lanes (a tenth idle at most)
+// and every operand is 64 MB or more, wide accesses are worth the fold: f32 [512, 16, 4096] 73 us and a thread per channel 87,
+// backwards 142 and 161; backwards in 16 bits too, [512, 16, 4096] bf16 82 and 101, [2000, 13, 1003] 81 and 84. Not forwards
+// (52 and 42), smaller ([128, 16, 4096] f32 backwards 34 and 32) or with idle lanes ([8000, 16, 260] bf16 backwards 139 and
+// 117).
+constexpr int64_t kNearlyATile = 13, kLarge = int64_t{64} << 20;
+bool short_scan_used(const hmr_tensor_desc *gate, const ScanLayout &layout, bool backward);
 // Whether the sequences are long enough for a scan, and not too many for a launch with a workgroup for every tile.
 bool scan_used(const hmr_tensor_desc *gate);
 // Bytes of workspace of either direction, whatever the operands' strides.

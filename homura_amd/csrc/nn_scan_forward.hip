@@ -36,6 +36,18 @@ bool scan_used(const hmr_tensor_desc *gate) {
                        kScanBlock);
 }
 
+bool short_scan_used(const hmr_tensor_desc *gate, const ScanLayout &layout, bool backward) {
+    const int64_t B = gate->sizes[0], T = gate->sizes[1], C = gate->sizes[2], size = dtype_size(gate->dtype);
+    if (!layout.adjacent || T < kNearlyATile || T > kShortest || size > 4 || (size == 2 && !backward)) return false;
+    bool used = false;
+    with_float_type(gate->dtype, [&](auto tag) {
+        using Shape = ShortShape<typename decltype(tag)::type>;
+        const int64_t blocks = Shape::blocks(C);
+        used = B * T * C * size >= kLarge && 10 * C >= 9 * blocks * Shape::kChannels && fits_launch(B * blocks, kScanBlock);
+    });
+    return used;
+}
+
 int64_t room_for(const hmr_tensor_desc *gate) {
     if (!scan_used(gate)) return 0;
     return 8 * most_of(gate, [&](auto shape) {
