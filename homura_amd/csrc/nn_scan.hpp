@@ -180,8 +180,9 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
     const bool folds = tid < CL && cj < t.c1;
     C carry = 0;  // of channel cj: the value that enters the tile, then the one that leaves it
     if (folds && t.k == 0 && a.entry.p != nullptr) carry = load_state<T>(a.entry.p, a.entry.at(t.b, cj), a.entry.wide);
-    // The lane's steps as maps, and their fold: what it adds is the state from zero exactly as steps one by one leave it
-    // (a zero times a factor that is not finite is NaN). The maps are computed again when the steps are run.
+    // The lane's steps as maps, and their fold: what it adds is the state from zero exactly as steps one by one leave it (a
+    // zero times a factor that is not finite is NaN, so that what follows such a step is never finite, though steps from
+    // another state might leave an infinity where the fold has NaN). The maps are computed again when the steps are run.
     auto map = [&](int i, int j, C &f, C &add) {
         const C z = now.gate[i].get(j);
         if constexpr (!BACK) {

@@ -47,7 +47,8 @@ const char *hmn_last_error(void);
  * A scan folds stretches of steps into (product of factors, state from zero), so a product of factors beyond the
  * computation type's range is not finite where step-by-step evaluation might be, and one too small for it is zero. Factors
  * of magnitude at most one, as gates are, never meet the first, and the second loses nothing of a state in any ordinary
- * range.
+ * range. From a step with a factor that is itself not finite on, no state of the channel is finite; which ones are infinite
+ * and which NaN depends on the grouping and may differ between `out` and `last`. The same holds backwards, from the end.
  */
 #define HMN_GATE_FACTOR 0
 #define HMN_GATE_SIGMOID 1
