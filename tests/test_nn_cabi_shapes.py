@@ -27,3 +27,20 @@ def test_a_workspace_query_of_any_size_is_answered():
             capi.check_nn(capi.nn.hmn_recurrence_workspace(byref(desc(dtype, *sizes, strides=[0, 0, 0])), byref(need)))
             assert need.value == 0, sizes
     refused(capi.nn.hmn_recurrence_workspace(byref(desc(capi.F32, 1 << 31, 1 << 31, 4, strides=[0, 0, 0])), byref(need)), "does not fit 64 bits")
+
+
+@pytest.mark.parametrize("dtype", [capi.BF16, capi.F32, capi.F64])
+def test_chained_scans_and_maps_need_a_workspace(dtype):
+    need = c_int64(-1)
+    for sizes in ((2, 100000, 24), (1, 5000, 24), (8, 2048, 4096)):
+        capi.check_nn(capi.nn.hmn_recurrence_workspace(byref(desc(dtype, *sizes)), byref(need)))
+        assert need.value > 0, sizes
+    for backward in (0, 1):
+        for sizes, groups in (((4, 20000, 24), 4), ((16, 4096, 320), 32), ((1, 70, 8), 1)):
+            capi.check_nn(capi.nn.hmn_group_norm_workspace(byref(desc(dtype, *sizes)), groups, backward, byref(need)))
+            assert need.value > 0, sizes
+    # Tokens leave sums of their own for the weights' gradients, and nothing forwards.
+    capi.check_nn(capi.nn.hmn_group_norm_workspace(byref(desc(dtype, 16384, 1, 4096)), 32, 1, byref(need)))
+    assert need.value > 0
+    capi.check_nn(capi.nn.hmn_group_norm_workspace(byref(desc(dtype, 16384, 1, 4096)), 32, 0, byref(need)))
+    assert need.value == 0
