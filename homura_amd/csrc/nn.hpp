@@ -85,6 +85,24 @@ __device__ __forceinline__ void exp_parts(float v, float &e, float &t) {
     if constexpr (sizeof(T) > 2) t = fminf(fma_(p, -kLn2Rest, fma_(p, -kLn2, v)), 1.0f);
 }
 
+// sigmoid(z) and 1 - sigmoid(z), each to within seven half steps of its own, |z| more for the smaller one beside 16-bit
+// sequences (exp_parts; below 2^-126 it is zero): the smaller of the two comes from exp(-|z|) itself, not from a subtraction.
+template <class T>
+__device__ __forceinline__ void sigmoid_pair(float z, float &a, float &rest) {
+    float e, t;
+    exp_parts<T>(-fabsf(z), e, t);
+    if constexpr (sizeof(T) > 2) e = fma_(e, t, e);
+    const float q = __builtin_amdgcn_rcpf(1.0f + e), r = e * q;
+    a = z < 0.0f ? r : q;
+    rest = z < 0.0f ? q : r;
+}
+template <class T>
+__device__ __forceinline__ void sigmoid_pair(double z, double &a, double &rest) {
+    const double e = exp(-fabs(z)), q = 1.0 / (1.0 + e), r = e * q;
+    a = z < 0.0 ? r : q;
+    rest = z < 0.0 ? q : r;
+}
+
 // V elements of type T as memory holds them, moved in accesses of up to 16 bytes. The vectors need no more alignment than
 // an element has (global accesses of this target take any), so a row of odd length or an odd start costs a few split
 // lines, not another kernel.

@@ -51,24 +51,6 @@ struct RecurrenceArgs {
     }
 };
 
-// sigmoid(z) and 1 - sigmoid(z), each to within seven half steps of its own, |z| more for the smaller one beside 16-bit
-// sequences (exp_parts; below 2^-126 it is zero): the smaller of the two comes from exp(-|z|) itself, not from a subtraction.
-template <class T>
-__device__ __forceinline__ void sigmoid_pair(float z, float &a, float &rest) {
-    float e, t;
-    exp_parts<T>(-fabsf(z), e, t);
-    if constexpr (sizeof(T) > 2) e = fma_(e, t, e);
-    const float q = __builtin_amdgcn_rcpf(1.0f + e), r = e * q;
-    a = z < 0.0f ? r : q;
-    rest = z < 0.0f ? q : r;
-}
-template <class T>
-__device__ __forceinline__ void sigmoid_pair(double z, double &a, double &rest) {
-    const double e = exp(-fabs(z)), q = 1.0 / (1.0 + e), r = e * q;
-    a = z < 0.0 ? r : q;
-    rest = z < 0.0 ? q : r;
-}
-
 // The factor and the addend of a step.
 template <class T, int FORM, class C>
 __device__ __forceinline__ void factor_and_input(C gate, C input, C &factor, C &addend) {
