@@ -63,7 +63,9 @@ __global__ void __launch_bounds__(kBlock) rows_kernel(RowsArgs s) {
 #pragma unroll
         for (int m = 0; m < M; ++m) fetch_weights(m, keep_w[m], keep_b[m]);
     }
-    // The sums of both over a group's lanes: moments in f64, the gradient's two sums in the computation type.
+    // The sums of both over a group's lanes: moments in f64, the gradient's two sums in the computation type (V additions in a
+    // row for each of a lane's M vectors, then those and the lanes pairwise or nearly so: in f32 as good as a pairwise sum, and
+    // in f64 [8192, 4096] f16 took 55 us for 52).
     using A = std::conditional_t<BACK, C, double>;
     __shared__ A wide_sums[2][kWaves];
     auto group_sums = [&](A &x, A &y) {

@@ -355,9 +355,9 @@ template <class T>
 using ShortShape = ScanShape<T, kVector<T>, kSlots, 1>;
 template <class T, bool BACK>
 using LongShape = ScanShape<T, kVector<T>, BACK ? 32 : 16, BACK ? 4 : 6>;
-// Of few vectors of channels: the lanes that those would leave idle go along the sequence ([240, 8324, 8] f32 87 us, 387
+// Of few vectors of channels: the lanes that those would leave idle go along the sequence ([240, 8324, 8] f32 101 us, 450
 // with the long shape; [75, 906, 39] bf16 19 and 37). Of up to four blocks of channels (two backwards) too, where the long
-// shape would need several tiles ([240, 8324, 128] bf16 508 us and 638; backwards, 64 channels, 416 and 542, but 128
+// shape would need several tiles ([240, 8324, 128] bf16 504 us and 637; backwards, 64 channels, 415 and 542, but 128
 // channels 799 and 662).
 template <class T>
 using NarrowShape = ScanShape<T, kVector<T>, 128, 4>;

@@ -103,7 +103,7 @@ hmr_status hmn_group_norm(hmr_context_t ctx, const hmr_tensor_desc *out, const h
  * d = grad * act'(z) and <.> the mean over a group's elements:
  *   d_bias = sum over n, s of d,  d_weight = sum over n, s of d * hat
  *   d_src = rstd * (weight * d - <weight * d> - hat * <weight * d * hat>)
- * d_weight and d_bias [C] may be NULL (not wanted) and have weight's type (src's where weight is NULL) or F32.
+ * d_weight and d_bias [C] may be NULL (not wanted) and have src's type or F32, each for itself.
  * The derivative of RELU at zero is zero.
  */
 hmr_status hmn_group_norm_backward(hmr_context_t ctx, const hmr_tensor_desc *d_src,
