@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(kBlock) channel_sums_kernel(MapsArgs m) {
     const Place<V> at(a, m.p);
     Walk<T, V, 2> walk(at, a, m.p, a.src, a.grad);
     constexpr bool kRuns = sizeof(C) == 4;
+    static_assert(kMostRun % kAtOnce == 0, "a run ends where the walk's steps end");
     C sum[V], sum_h[V], all[kRuns ? V : 1], all_h[kRuns ? V : 1];
     int run = 0;
 #pragma unroll

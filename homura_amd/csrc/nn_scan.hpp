@@ -298,7 +298,9 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
 #pragma unroll
     for (int j = 0; j < V; ++j) e[j] = t.lane_on ? slot_u[r][t.at + j] : C(0);
     if (t.lane_on) {
-        char *const to = BACK && sizeof(T) < sizeof(C) && a.d_gate_wide ? base_of(t, a.d_gate, 0, sizeof(C)) : base(t, BACK ? a.d_gate : a.out), *const to_input = BACK ? base(t, a.d_input) : nullptr;
+        const bool wide_gate = BACK && sizeof(T) < sizeof(C) && a.d_gate_wide;
+        char *const to = base_of(t, BACK ? a.d_gate : a.out, 0, wide_gate ? sizeof(C) : sizeof(T));
+        char *const to_input = BACK ? base(t, a.d_input) : nullptr;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             Vec<T, V> out;
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kScanBlock) scan_kernel(ScanArgs s) {
                     if constexpr (FORM == HMN_GATE_SIGMOID) x = now.input[i].get(j);
                     e[j] = step_back<T, FORM>(now.gate[i].get(j), x, g, before, dg[j], dx[j]);
                 }
-                if (sizeof(T) < sizeof(C) && a.d_gate_wide) {
+                if (wide_gate) {
                     Vec<C, V> wide;
                     wide.round(dg);
                     wide.only(t.has(i));
